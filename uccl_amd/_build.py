@@ -32,13 +32,22 @@ SOURCES = [
     CSRC / "ep" / "ep_kernels.hip",
     CSRC / "ep" / "ep_buffer.cpp",
     CSRC / "ep" / "ep_proxy.cpp",
+    CSRC / "ep" / "expert_route.hip",
+    CSRC / "ep" / "expert_gemm.hip",
+    CSRC / "ep" / "expert_act.hip",
     CSRC / "ukernel" / "ukernel.cpp",
     CSRC / "ukernel" / "uk_device.hip",
     CSRC / "p2p" / "compress.cpp",
     CSRC / "p2p" / "gpu_codec.hip",
     CSRC / "core" / "trace.cpp",
+    CSRC / "bindings" / "expert_ops.cpp",
     CSRC / "bindings" / "module.cpp",
 ]
+
+# Some packed FP32 forms that hipcc makes by itself from scalar float code have
+# given wrong results on gfx950; keep them out of every device build (hipcc's
+# host pass warns that it does not know the feature).
+DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 EXT_NAME = "_C" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so")
 
@@ -83,7 +92,7 @@ def build_plugin(verbose: bool = False) -> Path:
     shim_check = plugdir / "libuccl_nccl.so"
     shim_deps = [CSRC / "nccl_shim" / "nccl_shim.cpp",
                  CSRC / "collective" / "kernels.hip",
-                 CSRC / "collective" / "communicator.cpp"]
+                 CSRC / "collective" / "communicator.cpp", Path(__file__)]
     if (not _stale(target, deps) and not _stale(harness, deps)
             and not _stale(capi, capi_srcs + deps)
             and not _stale(shim_check, shim_deps)):
@@ -131,10 +140,11 @@ def build_plugin(verbose: bool = False) -> Path:
                  CSRC / "collective" / "kernels.hip",
                  CSRC / "collective" / "communicator.cpp"]
     shim_hdrs = list((CSRC / "collective").glob("*.h")) + [
-        CSRC / "device" / "primitives.h"]
+        CSRC / "device" / "primitives.h", Path(__file__)]
     if _stale(shim, shim_srcs + shim_hdrs + deps):
         cmd = [HIPCC, "-O3", "-std=c++17", "-fPIC", "-shared",
-               f"--offload-arch={GPU_ARCH}"] + [str(x) for x in shim_srcs] + [
+               f"--offload-arch={GPU_ARCH}", *DEVICE_FLAGS] + [
+                   str(x) for x in shim_srcs] + [
                "-o", str(shim), "-pthread", f"-L{ROCM}/lib", "-lamdhip64",
                f"-Wl,-rpath,{ROCM}/lib"]
         if verbose:
@@ -175,7 +185,8 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     """Compile the extension in-tree. Returns the path to the built .so."""
     target = PKG_DIR / EXT_NAME
     incs, libdir = _torch_paths()
-    headers = list(CSRC.rglob("*.h"))
+    # the flags above are an input of the build as well
+    headers = list(CSRC.rglob("*.h")) + [Path(__file__)]
     sources = [s for s in SOURCES if s.exists()]
     if not force and not _stale(target, sources + headers):
         return target
@@ -195,6 +206,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         "-D_GLIBCXX_USE_CXX11_ABI=1",
         "-fno-gpu-rdc",
         "-Wno-unused-result",
+        *DEVICE_FLAGS,
         f"-I{py_inc}",
     ] + [f"-I{i}" for i in incs]
 

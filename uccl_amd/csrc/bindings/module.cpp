@@ -26,6 +26,7 @@ namespace py = pybind11;
 
 namespace uccl {
 void register_pg_backend(pybind11::module_& m);
+void register_expert_ops(pybind11::module_& m);
 }
 
 using uccl::Communicator;
@@ -72,6 +73,7 @@ PYBIND11_MODULE(_C, m) {
   m.doc() = "uccl_amd native engine (MI355X / gfx950)";
 
   uccl::register_pg_backend(m);
+  uccl::register_expert_ops(m);
 
   m.def("device_count", [] {
     int n = 0;

@@ -181,7 +181,15 @@ class Buffer:
     low_latency_combine = combine
 
 
+_EXPERT_OPS = ("route", "route_grad", "expert_matmul", "expert_weight_grad",
+               "expert_swiglu", "expert_swiglu_grad")
+
+
 def __getattr__(name):
+    if name in _EXPERT_OPS:
+        from uccl_amd.ep import experts
+
+        return getattr(experts, name)
     if name in ("ElasticBuffer", "MembershipChanged", "expert_rank_table"):
         from uccl_amd.ep import elastic
 

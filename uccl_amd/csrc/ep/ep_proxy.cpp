@@ -4,9 +4,11 @@
 #include <sched.h>
 #include <unistd.h>
 
+#include <algorithm>
 #include <chrono>
-
 #include <cstring>
+#include <map>
+#include <mutex>
 #include <thread>
 
 #include "../core/env.h"
@@ -94,9 +96,32 @@ struct TimedFlowLock {
   ~TimedFlowLock() { m.unlock(); }
 };
 
+// Lane copies must never queue behind the user's spin-wait kernels. HIP
+// gives a new stream a hardware queue of its own while it has one left
+// (GPU_MAX_HW_QUEUES, 4 by default) and lets further ones share, the null
+// stream's queue among them: with 5 lanes (world 4) and 4 queues a lane's
+// copy sat behind the dispatch wait that needed it, until that timed out.
+// So lanes take turns on at most queues - 1 streams, which live as long as
+// the process: a destroyed one would hand its queue to somebody else.
+static hipStream_t lane_stream(int device) {
+  static std::mutex mu;
+  static std::map<int, std::pair<std::vector<hipStream_t>, size_t>> pools;
+  std::lock_guard<std::mutex> g(mu);
+  auto& [streams, next] = pools[device];
+  size_t const most = static_cast<size_t>(
+      std::max<int64_t>(1, env_int("GPU_MAX_HW_QUEUES", 4) - 1));
+  if (streams.size() < most) {
+    hipStream_t s = nullptr;
+    UCCL_CHECK_HIP(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
+    streams.push_back(s);
+    return s;
+  }
+  return streams[next++ % most];
+}
+
 EpProxy::Lane::Lane(int device, size_t bytes) {
   UCCL_CHECK_HIP(hipSetDevice(device));
-  UCCL_CHECK_HIP(hipStreamCreateWithFlags(&stream, hipStreamNonBlocking));
+  stream = lane_stream(device);
   UCCL_CHECK_HIP(hipHostMalloc(&buf, bytes));
   UCCL_CHECK_HIP(hipHostMalloc(&buf2, bytes));
 }
@@ -104,7 +129,6 @@ EpProxy::Lane::Lane(int device, size_t bytes) {
 EpProxy::Lane::~Lane() {
   if (buf) (void)hipHostFree(buf);
   if (buf2) (void)hipHostFree(buf2);
-  if (stream) (void)hipStreamDestroy(stream);
 }
 
 EpProxy::EpProxy(const EpView& view, void* heap, D2HRing* ring_host,

@@ -62,6 +62,7 @@ class EpProxy {
   // Per-thread pinned staging + non-blocking stream: the ring thread,
   // the combine-tx thread, and every per-peer rx thread run concurrently
   // and must never share host staging (corruption observed at world=4).
+  // Lanes may share a stream, and do not own it (lane_stream()).
   struct Lane {
     void* buf = nullptr;
     void* buf2 = nullptr;  // double buffer: D2H of chunk i+1 overlaps the

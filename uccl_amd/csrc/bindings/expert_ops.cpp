@@ -119,7 +119,8 @@ ep::SlotRows rows_of(at::Tensor const& x, OptTensor const& counts) {
   TORCH_CHECK(experts >= 1 && experts <= ep::kMaxSlotExperts,
               "uccl_amd: 1 to ", ep::kMaxSlotExperts, " experts, got ",
               experts);
-  TORCH_CHECK(slots < (int64_t(1) << 31), "uccl_amd: too many slots");
+  TORCH_CHECK(experts * slots < (int64_t(1) << 31),
+              "uccl_amd: too many slots");
   int64_t sources = 1;
   if (counts) {
     check_on(*counts, x, "counts");
@@ -131,6 +132,9 @@ ep::SlotRows rows_of(at::Tensor const& x, OptTensor const& counts) {
                 ", expected [", experts, ", sources]");
     check_dense(*counts, "counts");
     sources = counts->size(1);
+    TORCH_CHECK(experts * sources <= ep::kMaxSlotCells,
+                "uccl_amd: at most ", ep::kMaxSlotCells,
+                " counts, got ", experts * sources);
     TORCH_CHECK(slots % sources == 0, "uccl_amd: ", slots,
                 " slots do not divide among ", sources, " sources");
   }
@@ -310,6 +314,8 @@ void expert_matmul(at::Tensor x, at::Tensor w, OptTensor counts,
                 "uccl_amd: 8-bit operands need x_scales and w_scales");
     TORCH_CHECK(k % 128 == 0,
                 "uccl_amd: 8-bit products need k % 128 == 0, got ", k);
+    TORCH_CHECK(n == 1 || w.stride(1) < (int64_t(1) << 24),
+                "uccl_amd: rows of 8-bit weights are less than 16 MiB apart");
     TORCH_CHECK(a.out_elem != Elem::kF32,
                 "uccl_amd: 8-bit products give bfloat16 or float16: the 8-bit "
                 "matrix unit does not keep the precision of float32");

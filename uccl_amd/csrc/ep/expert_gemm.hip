@@ -7,13 +7,13 @@
 //   weight gradient  dw[n, k] = sum_m g[m, n] x[m, k], over the valid rows
 //
 // One kernel computes D[p, q] = sum_c P[p, c] Q[q, c] tile by tile with MFMA
-// 16x16 instructions; a lane then holds 4 consecutive p of one q, so p is the
+// 16x16 instructions; a lane then holds consecutive p of one q, so p is the
 // contiguous dimension of the result: P = w, Q = x for a product, P = x^T,
 // Q = g^T for the weight gradient.
 //
-// The tile's operands go from memory to LDS in steps of 128 bytes (direct
+// A tile's operands go from memory to LDS in steps of 128 bytes (direct
 // operands, contiguous along c) or 64 rows (turned operands, contiguous along
-// p or q; read back through the transposing LDS load), double-buffered, by
+// p or q; read back through the transposing LDS load), in two stages, by
 // loads that write LDS without passing registers. Each lane forms its own
 // address, so the valid rows of all sources are gathered on the way: a tile
 // is full of valid rows wherever they lie.
@@ -25,6 +25,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../core/log.h"
 #include "../device/primitives.h"
@@ -46,60 +47,97 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr int kStep = 128;  // bytes of the contraction in a stage, a row
 
 // 16 bytes of zeros: where lanes behind the contraction's end load from.
 __device__ const int4 zero_page = {0, 0, 0, 0};
 
-// Load 16 (4) bytes of each lane from its own address to LDS at `lds` + lane
-// * 16 (* 4). The instruction has no register result; the caller waits with
-// wait_loads() and a barrier before the LDS is read.
-__device__ __forceinline__ void lds_load16(void const* g, uint32_t lds) {
+// --- loads to LDS ----------------------------------------------------------
+// Each lane loads 16 (4) bytes from its own address to LDS at `lds` + kAt +
+// lane * 16 (* 4), where `on` is not 0. `on` and `lds` are uniform. The
+// instruction has no register result; the wave waits for it in a barrier
+// below before the LDS is read. The branch is inside the statement so that it
+// does not cut the block that the compiler schedules.
+
+template <int kAt>
+__device__ __forceinline__ void lds_load16(int on, char const* base,
+                                           uint32_t offset, uint32_t lds) {
   asm volatile(
-      "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+      "s_cmp_eq_u32 %4, 0\n\ts_cbranch_scc1 1f\n\ts_add_u32 m0, %2, %3\n\t"
+      "s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n1:"
       :
-      : "v"(g), "s"(lds)
-      : "memory", "m0");
+      : "v"(offset), "s"(base), "s"(lds), "n"(kAt), "s"(on)
+      : "memory", "m0", "scc");
 }
-__device__ __forceinline__ void lds_load4(void const* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
-               :
-               : "v"(g), "s"(lds)
-               : "memory", "m0");
+template <int kAt>
+__device__ __forceinline__ void lds_load16(int on, char const* g,
+                                           uint32_t lds) {
+  asm volatile(
+      "s_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 1f\n\ts_add_u32 m0, %1, %2\n\t"
+      "s_nop 0\n\tglobal_load_lds_dwordx4 %0, off\n1:"
+      :
+      : "v"(g), "s"(lds), "n"(kAt), "s"(on)
+      : "memory", "m0", "scc");
+}
+__device__ __forceinline__ void lds_load4(int on, char const* g,
+                                          uint32_t lds) {
+  asm volatile(
+      "s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 1f\n\ts_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\tglobal_load_lds_dword %0, off\n1:"
+      :
+      : "v"(g), "s"(lds), "s"(on)
+      : "memory", "m0", "scc");
 }
 
-// Every load to LDS of this wave has landed, every LDS read of it is done,
-// and so for the other waves of the block.
-__device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// This wave's LDS reads are done and its loads and stores have landed, all
+// but the last `left` (0, kMore or kMost; uniform); and so for the other waves
+// of the block.
+template <int kMore, int kMost>
+__device__ __forceinline__ void stage_barrier(int left) {
+  asm volatile(
+      "s_cmp_lt_i32 %2, %1\n\ts_cbranch_scc0 2f\n\t"
+      "s_cmp_lt_i32 %2, %0\n\ts_cbranch_scc0 1f\n\t"
+      "s_waitcnt vmcnt(0)\n1:\n\ts_waitcnt vmcnt(%0)\n2:\n\t"
+      "s_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_barrier" ::"n"(kMore),
+      "n"(kMost), "s"(left)
+      : "memory", "scc");
 }
 
 __device__ __forceinline__ uint32_t lds_addr(void const* p) {
   return static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)p));
 }
-
-__device__ __forceinline__ int clamp_count(SlotRows const& r, int i) {
-  return r.counts ? min(max(r.counts[i], 0), r.length) : r.length;
+template <typename T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+  return *reinterpret_cast<__attribute__((address_space(3))) T const*>(at);
+}
+__device__ __forceinline__ i16x4 lds_read_turned(uint32_t at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      reinterpret_cast<__attribute__((address_space(3))) i16x4*>(at));
 }
 
-__device__ __forceinline__ int rows_of(SlotRows const& r, int e) {
-  int n = 0;
-  for (int s = 0; s < r.sources; ++s) n += clamp_count(r, e * r.sources + s);
-  return n;
+__device__ __forceinline__ int uniform(int v) {
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
-// Slot of the i-th valid row of expert e; i < rows_of(e).
-__device__ __forceinline__ int slot_of(SlotRows const& r, int e, int i) {
-  i = max(i, 0);
-  for (int s = 0; s < r.sources; ++s) {
-    int const n = clamp_count(r, e * r.sources + s);
-    if (i < n) return s * r.length + i;
-    i -= n;
+// -1 where a < b, else 0, for uniform operands: a condition that stays in
+// scalar registers, where the statements above want it.
+__device__ __forceinline__ int before(int a, int b) {
+  int r;
+  asm("s_cmp_lt_i32 %1, %2\n\ts_cselect_b32 %0, -1, 0"
+      : "=s"(r)
+      : "s"(a), "s"(b)
+      : "scc");
+  return r;
+}
+
+template <int kAt, int kEnd, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  if constexpr (kAt < kEnd) {
+    f(std::integral_constant<int, kAt>{});
+    unrolled<kAt + 1, kEnd>(f);
   }
-  return 0;
 }
 
 struct GemmArgs {
@@ -109,9 +147,10 @@ struct GemmArgs {
   char* out;
   // bytes
   int64_t p_expert, p_row, q_expert, q_row, out_expert, out_row;
-  int np;       // extent of p
-  int nq;       // extent of q (weight gradient only; else the valid rows)
-  int depth;    // contraction in elements (product only)
+  int np;     // extent of p
+  int nq;     // extent of q (weight gradient only; else the valid rows)
+  int depth;  // contraction in elements (product only)
+  bool wide;  // 8 results of a row can be stored together
   char const* q_scales;
   char const* p_scales;
   int64_t qs_expert, qs_row, ps_expert, ps_row;  // bytes
@@ -138,26 +177,149 @@ __device__ __forceinline__ f32x4 mfma8(i32x8 a, i32x8 b) {
 }
 
 template <Elem kOut>
-__device__ __forceinline__ void store4(char* at, f32x4 v, int n, bool wide) {
-  using T = std::conditional_t<
-      kOut == Elem::kF32, float,
-      std::conditional_t<kOut == Elem::kBF16, __hip_bfloat16, __half>>;
-  T* o = reinterpret_cast<T*>(at);
-  if (wide) {
-    struct alignas(4 * sizeof(T)) Four {
-      T v[4];
-    } four;
+using OutType = std::conditional_t<
+    kOut == Elem::kF32, float,
+    std::conditional_t<kOut == Elem::kBF16, __bf16, _Float16>>;
+
+// Store 8 results of a row, at a 16-byte boundary; or the first n of them.
+template <Elem kOut>
+__device__ __forceinline__ void store8(char* at, f32x4 a, f32x4 b) {
+  using T = OutType<kOut>;
+  struct alignas(16) Pack {
+    T v[16 / sizeof(T)];
+  };
+  Pack pack[sizeof(T) / 2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) four.v[j] = static_cast<T>(v[j]);
-    *reinterpret_cast<Four*>(o) = four;
-  } else {
+  for (int j = 0; j < 8; ++j)
+    pack[j * sizeof(T) / 16].v[j % (16 / sizeof(T))] =
+        static_cast<T>(j < 4 ? a[j % 4] : b[j % 4]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) o[j] = static_cast<T>(v[j]);
-  }
+  for (unsigned j = 0; j < sizeof(T) / 2; ++j)
+    reinterpret_cast<Pack*>(at)[j] = pack[j];
+}
+template <Elem kOut>
+__device__ __forceinline__ void store_few(char* at, f32x4 a, f32x4 b, int n) {
+  using T = OutType<kOut>;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n)
+      reinterpret_cast<T*>(at)[j] = static_cast<T>(j < 4 ? a[j % 4] : b[j % 4]);
 }
 
-// Tiles BP x BQ, WP x WQ waves, two stages.
+// --- the valid rows of all experts, in LDS ---------------------------------
+struct RowTable {
+  int end[kMaxSlotCells];        // [expert][source]: valid rows up to there
+  int tile_end[kMaxSlotExperts];  // tiles of rows up to and with the expert
+};
+
+__device__ __forceinline__ void fill_table(RowTable& t, SlotRows const& r,
+                                           int tile_rows) {
+  int const cells = r.experts * r.sources;
+  for (int i = threadIdx.x; i < cells; i += blockDim.x)
+    t.end[i] = r.counts ? min(max(r.counts[i], 0), r.length) : r.length;
+  __syncthreads();
+  for (int e = threadIdx.x; e < r.experts; e += blockDim.x) {
+    int n = 0;
+    for (int s = 0; s < r.sources; ++s) {
+      n += t.end[e * r.sources + s];
+      t.end[e * r.sources + s] = n;
+    }
+    t.tile_end[e] = (n + tile_rows - 1) / tile_rows;
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    int const lane = threadIdx.x;
+    int carry = 0;
+    for (int e0 = 0; e0 < r.experts; e0 += 64) {
+      int v = e0 + lane < r.experts ? t.tile_end[e0 + lane] : 0;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        int const o = __shfl_up(v, off);
+        if (lane >= off) v += o;
+      }
+      if (e0 + lane < r.experts) t.tile_end[e0 + lane] = carry + v;
+      carry += __shfl(v, 63);
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ int valid_rows(RowTable const& t, SlotRows const& r,
+                                          int e) {
+  return t.end[(e + 1) * r.sources - 1];
+}
+
+// Slot of the i-th valid row of expert e, i below valid_rows().
+__device__ __forceinline__ int slot_of(RowTable const& t, SlotRows const& r,
+                                       int e, int i) {
+  int begin = 0;
+  for (int s = 0; s < r.sources; ++s) {
+    int const end = t.end[e * r.sources + s];
+    if (i < end) return s * r.length + i - begin;
+    begin = end;
+  }
+  return 0;
+}
+
+struct Tile {
+  int e, p0, q0;
+  int valid;  // rows of the expert
+};
+
+// Tiles are counted expert by expert; in an expert, four rows of tiles at a
+// time, so that tiles near in order share both operands.
+template <Mode kMode, int BP, int BQ>
+__device__ __forceinline__ Tile find_tile(GemmArgs const& a,
+                                          RowTable const& t, int tile,
+                                          int tiles_p) {
+  int e, local, tiles_q;
+  if constexpr (kMode == Mode::kWeightGrad) {
+    tiles_q = (a.nq + BQ - 1) / BQ;
+    e = tile / (tiles_p * tiles_q);
+    local = tile - e * tiles_p * tiles_q;
+  } else {
+    int const row = tile / tiles_p;  // counted over all experts
+    int lo = 0, hi = a.rows.experts - 1;  // first e with row < tile_end[e]
+    while (lo < hi) {
+      int const mid = (lo + hi) >> 1;
+      if (row < t.tile_end[mid]) hi = mid;
+      else lo = mid + 1;
+    }
+    e = lo;
+    int const begin = e ? t.tile_end[e - 1] : 0;
+    tiles_q = t.tile_end[e] - begin;
+    local = tile - begin * tiles_p;
+  }
+  int const band = local / (4 * tiles_p) * 4;
+  int const in_band = local - band * tiles_p;
+  int const high = min(4, tiles_q - band);
+  Tile r;
+  r.e = uniform(e);
+  r.q0 = uniform((band + in_band % high) * BQ);
+  r.p0 = uniform(in_band / high * BP);
+  r.valid = uniform(valid_rows(t, a.rows, e));
+  return r;
+}
+
+constexpr int less(int a, int b) { return a < b ? a : b; }
+
+template <int kH>
+__device__ __forceinline__ i32x4 half(i32x8 v) {
+  return __builtin_shufflevector(v, v, kH * 4, kH * 4 + 1, kH * 4 + 2,
+                                 kH * 4 + 3);
+}
+
+// Tiles BP x BQ, WP x WQ waves of TP x TQ MFMA tiles, two stages.
+//
+// Places in LDS. Direct operands: a row of 128 bytes, its 16-byte chunk c at
+// place c ^ f(row), f taken from the row bits in which the 16 rows that a wave
+// reads together differ, so that these reads fall into different banks. Turned
+// operands: a row of the contraction, chunk c at place c ^ ((row & 3) << 2).
+// Q comes in two halves, of the first and the last half of each wave's rows.
+//
+// P rows are given to MFMA rows so that a lane's results of two tiles are 8
+// consecutive p: row m of tile i is p = 32 (i / 2) + 8 (m / 4) + 4 (i % 2) +
+// m % 4 of the wave's 64.
 template <Mode kMode, Elem kElem, Elem kOut, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   constexpr bool kWGrad = kMode == Mode::kWeightGrad;
@@ -167,317 +329,477 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   constexpr int kSize = k8 ? 1 : 2;
   constexpr int kDepth = kStep / kSize;  // contraction elements of a stage
   constexpr int kWaves = WP * WQ, kThreads = kWaves * 64;
-  constexpr int TP = BP / WP / 16, TQ = BQ / WQ / 16;  // 16x16 tiles of a wave
+  constexpr int RP = BP / WP, RQ = BQ / WQ;  // rows of a wave
+  constexpr int TP = RP / 16, TQ = RQ / 16, kT = TP * TQ;
   constexpr int kPBytes = BP * kStep, kQBytes = BQ * kStep;
-  constexpr int kScaleBytes = k8 ? BQ * 4 : 0;
-  constexpr int kStage = kPBytes + kQBytes + kScaleBytes;
-  constexpr int kPLoads = kPBytes / 1024 / kWaves;
+  constexpr int kStage = kPBytes + kQBytes;
+  constexpr int kPLoads = kPBytes / 1024 / kWaves;  // of a wave and stage
   constexpr int kQLoads = kQBytes / 1024 / kWaves;
+  constexpr int kHalf = kQLoads / 2;
+  constexpr int kFirst = kPLoads + kHalf, kLoads = kPLoads + kQLoads;
   static_assert(kPLoads * 1024 * kWaves == kPBytes, "P loads");
-  static_assert(kQLoads * 1024 * kWaves == kQBytes, "Q loads");
-  static_assert(!k8 || 128 % (BP / WP) == 0, "a wave stays in a scale block");
+  static_assert(kHalf * 2048 * kWaves == kQBytes, "Q loads");
+  constexpr int kOutSize = kOut == Elem::kF32 ? 4 : 2;
+  constexpr int kStores = kT * kOutSize / 4;  // of a whole tile
+  static_assert(kLoads + kStores < 64, "vmcnt");
+  static_assert(TP == 4 && TQ % 4 == 0, "places and stores");
+  static_assert(!k8 || (128 % RP == 0 && BQ <= kThreads), "scales");
+  // turned rows
+  constexpr int kPPitch = BP * 2, kQPitch = BQ;
 
   __shared__ __attribute__((aligned(1024))) char stages[2 * kStage];
-  __shared__ int tile_end[kWGrad ? 1 : kMaxSlotExperts];
-  __shared__ int slots[kWGrad ? 2 * kDepth : BQ];
+  __shared__ float q_scale[k8 ? 4 : 1][k8 ? BQ : 1];
+  __shared__ float p_scale[k8 ? 4 : 1][k8 ? 64 : 1];
+  __shared__ RowTable table;
+  // rows of a tile: of the last, whose results are stored, of this one and of
+  // the next; weight gradient: rows of a stage, 4 stages in a ring
+  __shared__ int slots[kWGrad ? 4 : 3][kWGrad ? kDepth : BQ];
 
-  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int const wave = uniform(threadIdx.x >> 6);
   int const lane = threadIdx.x & 63;
   int const wp = wave % WP, wq = wave / WP;
   uint32_t const lds0 = lds_addr(stages);
 
-  // --- tiles of all experts ------------------------------------------------
   int const tiles_p = (a.np + BP - 1) / BP;
-  int total;
-  if constexpr (kWGrad) {
-    total = a.rows.experts * tiles_p * ((a.nq + BQ - 1) / BQ);
-  } else {
-    for (int e = threadIdx.x; e < a.rows.experts; e += kThreads)
-      tile_end[e] = (rows_of(a.rows, e) + BQ - 1) / BQ * tiles_p;
-    __syncthreads();
-    if (wave == 0) {
-      int carry = 0;
-      for (int e0 = 0; e0 < a.rows.experts; e0 += 64) {
-        int v = e0 + lane < a.rows.experts ? tile_end[e0 + lane] : 0;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          int const o = __shfl_up(v, off);
-          if (lane >= off) v += o;
-        }
-        if (e0 + lane < a.rows.experts) tile_end[e0 + lane] = carry + v;
-        carry += __shfl(v, 63);
-      }
-    }
-    __syncthreads();
-    total = tile_end[a.rows.experts - 1];
-  }
+  fill_table(table, a.rows, kWGrad ? 1 : BQ);
+  int const total =
+      uniform(kWGrad ? a.rows.experts * tiles_p * ((a.nq + BQ - 1) / BQ)
+                     : table.tile_end[a.rows.experts - 1] * tiles_p);
+  // Blocks are handed to the 8 XCDs in turn. Each round of tiles is cut into
+  // one run for each XCD, so that the blocks that share an L2 share operands,
+  // and all of the card works on neighbouring tiles, whose operands stay in
+  // the last-level cache.
+  int tile = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (tile >= total) return;
 
-  // Blocks are handed to the 8 XCDs in turn; each XCD gets a contiguous run
-  // of tiles, so that the blocks that share an L2 share operands.
-  int const per_xcd = (total + 7) / 8;
-  int const xcd = blockIdx.x & 7;
-  for (int i = blockIdx.x >> 3; i < per_xcd; i += gridDim.x >> 3) {
-    int const tile = xcd * per_xcd + i;
-    if (tile >= total) break;
+  // --- this lane's part of the loads ---------------------------------------
+  // P: loads wave * kPLoads on of the stage's; Q: wave * kHalf on of a half's.
+  auto p_row = [&](int j) {
+    int const at = (wave * kPLoads + j) * 64 + lane;
+    return kPTurned ? at / (kPPitch / 16) : at >> 3;
+  };
+  auto p_chunk = [&](int j) {
+    int const at = (wave * kPLoads + j) * 64 + lane, row = p_row(j);
+    if (kPTurned) return (at % (kPPitch / 16)) ^ ((row & 3) << 2);
+    return (at & 7) ^ (((row >> 1) & 1) | (((row >> 3) & 3) << 1));
+  };
+  auto q_row = [&](int j) {  // in the half
+    int const at = (wave * kHalf + j % kHalf) * 64 + lane;
+    return kQTurned ? at / (kQPitch / 16) : at >> 3;
+  };
+  auto q_chunk = [&](int j) {
+    int const at = (wave * kHalf + j % kHalf) * 64 + lane, row = q_row(j);
+    if (kQTurned)
+      return (at % (kQPitch / 16)) ^ (((row & 3) << 2) & (kQPitch / 16 - 1));
+    return (at & 7) ^ ((row >> 1) & 7);
+  };
+  // row (or column) of the tile that place r of half h belongs to
+  auto q_of = [&](int h, int r) {
+    return r / (RQ / 2) * RQ + h * (RQ / 2) + r % (RQ / 2);
+  };
 
-    // --- which tile --------------------------------------------------------
-    int e, local, tiles_q, valid;
-    if constexpr (kWGrad) {
-      tiles_q = (a.nq + BQ - 1) / BQ;
-      e = tile / (tiles_p * tiles_q);
-      local = tile % (tiles_p * tiles_q);
-      valid = rows_of(a.rows, e);
-    } else {
-      int lo = 0, hi = a.rows.experts - 1;  // first e with tile < tile_end[e]
-      while (lo < hi) {
-        int const mid = (lo + hi) >> 1;
-        if (tile < tile_end[mid]) hi = mid;
-        else lo = mid + 1;
-      }
-      e = lo;
-      int const begin = e ? tile_end[e - 1] : 0;
-      local = tile - begin;
-      tiles_q = (tile_end[e] - begin) / tiles_p;
-      valid = rows_of(a.rows, e);
-    }
-    e = __builtin_amdgcn_readfirstlane(e);
-    // four rows of tiles at a time, so that tiles near in order share both
-    // operands
-    int const band = local / (4 * tiles_p) * 4;
-    int const in_band = local - band * tiles_p;
-    int const high = min(4, tiles_q - band);
-    int const q0 = (band + in_band % high) * BQ;
-    int const p0 = in_band / high * BP;
+  char const* const zeros = reinterpret_cast<char const*>(&zero_page);
+  char const* p_base = nullptr;
+  uint32_t p_off[kPLoads];
+  char const* p_at[kPLoads];
+  char const* q_at[kQLoads];
+  char const* scale_at = nullptr;
+  int steps = 0, depth = 0;
 
-    __syncthreads();  // slots and stages of the last tile are no longer read
-    if constexpr (!kWGrad) {
-      for (int j = threadIdx.x; j < BQ; j += kThreads)
-        slots[j] = slot_of(a.rows, e, min(q0 + j, valid - 1));
-    } else {
-      if (threadIdx.x < kDepth && threadIdx.x < valid)
-        slots[threadIdx.x] = slot_of(a.rows, e, threadIdx.x);
-    }
-    __syncthreads();
-
-    // --- loads of a stage --------------------------------------------------
-    char const* const pe = a.p + e * a.p_expert;
-    char const* const qe = a.q + e * a.q_expert;
-    int const depth = kWGrad ? valid : a.depth;
-    int const steps = (depth + kDepth - 1) / kDepth;
-    char const* const zeros = reinterpret_cast<char const*>(&zero_page);
-
-    // Direct operand: a row of 128 bytes, 16-byte chunk c at place c ^ (row &
-    // 7). Turned operand: a row of B * 2 bytes, chunk c at place c ^ turn(row).
-    auto turn = [](int row) { return ((row & 3) | ((row >> 1) & 4)) << 1; };
-
-    char const* p_at[kPLoads];
-    char const* q_at[kQLoads];
+  // addresses of a tile's first stage
+  auto set_tile = [&](Tile const& t, int turn) {
+    char const* const pe = a.p + t.e * a.p_expert;
+    char const* const qe = a.q + t.e * a.q_expert;
+    depth = kWGrad ? t.valid : a.depth;
+    steps = uniform((depth + kDepth - 1) / kDepth);
+    // Rows of weights lie within 32 bits of the tile's first; gathered rows
+    // need not.
+    p_base = pe + static_cast<int64_t>(t.p0) * a.p_row;
 #pragma unroll
     for (int j = 0; j < kPLoads; ++j) {
-      int const at = (wave * kPLoads + j) * 64 + lane;
-      if constexpr (!kPTurned) {
-        int const row = at >> 3, c = (at & 7) ^ (row & 7);
-        p_at[j] = pe + static_cast<int64_t>(min(p0 + row, a.np - 1)) * a.p_row +
-                  c * 16;
-      } else {
-        int const row = at / (BP / 8), c = (at % (BP / 8)) ^ turn(row);
-        // a chunk behind the last column gives results that are not stored
-        int const col = min(p0 + c * 8, a.np - 8);
-        p_at[j] = pe + static_cast<int64_t>(kWGrad ? 0 : row) * a.p_row +
-                  static_cast<int64_t>(col) * 2;
-      }
+      if constexpr (k8)
+        p_off[j] = static_cast<uint32_t>(min(p_row(j), a.np - 1 - t.p0)) *
+                       static_cast<uint32_t>(a.p_row) +
+                   p_chunk(j) * 16;
+      else if constexpr (!kPTurned)
+        p_at[j] = pe +
+                  static_cast<int64_t>(min(t.p0 + p_row(j), a.np - 1)) *
+                      a.p_row +
+                  p_chunk(j) * 16;
+      else  // columns behind the last give results that are not stored
+        p_at[j] = pe + static_cast<int64_t>(kWGrad ? 0 : p_row(j)) * a.p_row +
+                  min(t.p0 + p_chunk(j) * 8, a.np - 8) * 2;
     }
 #pragma unroll
     for (int j = 0; j < kQLoads; ++j) {
-      int const at = (wave * kQLoads + j) * 64 + lane;
       if constexpr (!kQTurned) {
-        int const row = at >> 3, c = (at & 7) ^ (row & 7);
-        q_at[j] = qe + static_cast<int64_t>(slots[row]) * a.q_row + c * 16;
+        int const row = q_of(j / kHalf, q_row(j));
+        q_at[j] = qe + static_cast<int64_t>(slots[turn][row]) * a.q_row +
+                  q_chunk(j) * 16;
       } else {
-        int const row = at / (BQ / 8), c = (at % (BQ / 8)) ^ turn(row);
-        int const col = min(q0 + c * 8, a.nq - 8);
-        q_at[j] = qe + static_cast<int64_t>(col) * 2;
+        int const col = t.q0 + q_of(j / kHalf, q_chunk(j) * 8);
+        q_at[j] = qe + min(col, a.nq - 8) * 2;
       }
     }
-    char const* s_at = nullptr;
     if constexpr (k8) {
-      int const row = (wave % (BQ / 64)) * 64 + lane;
-      s_at = a.q_scales + e * a.qs_expert +
-             static_cast<int64_t>(slots[row]) * a.qs_row;
+      if (wave < BQ / 64) {
+        scale_at = a.q_scales + t.e * a.qs_expert +
+                   static_cast<int64_t>(slots[turn][threadIdx.x % BQ]) *
+                       a.qs_row;
+      } else {
+        int const block = min(t.p0 + min(lane, BP / 128 - 1) * 128, a.np - 1) / 128;
+        scale_at = a.p_scales + t.e * a.ps_expert + block * a.ps_row;
+      }
     }
+  };
 
-    auto load_stage = [&](int step) {
-      uint32_t const base = lds0 + (step & 1) * kStage;
-#pragma unroll
-      for (int j = 0; j < kPLoads; ++j) {
-        int const at = (wave * kPLoads + j) * 64 + lane;
+  uint32_t const my_p = lds0 + wave * kPLoads * 1024;
+  uint32_t const my_q = lds0 + kPBytes + wave * kHalf * 1024;
+  // Load n of stage `step`: P, then the two halves of Q.
+  auto load_part = [&](auto n, int on, int step)
+                       __attribute__((always_inline)) {
+    constexpr int j = decltype(n)::value;
+    uint32_t const buf = (step & 1) * kStage;
+    if constexpr (j < kPLoads) {
+      if constexpr (k8) {
+        lds_load16<j * 1024>(on, p_base, p_off[j], my_p + buf);
+        if (j == kPLoads - 1) p_base += kStep;
+      } else {
         char const* g;
         if constexpr (!kPTurned) {
-          int const c = (at & 7) ^ ((at >> 3) & 7);
-          int const left = a.depth * kSize - step * kStep - c * 16;
-          g = left > 0 ? p_at[j] + static_cast<int64_t>(step) * kStep : zeros;
+          g = step * kStep + p_chunk(j) * 16 < depth * kSize ? p_at[j] : zeros;
+          p_at[j] += kStep;
         } else {
-          int const row = step * kDepth + at / (BP / 8);
-          if constexpr (kWGrad)
-            g = row < depth
-                    ? p_at[j] + static_cast<int64_t>(
-                                    slots[(step & 1) * kDepth +
-                                          at / (BP / 8)]) *
-                                    a.p_row
-                    : zeros;
-          else
-            g = row < depth ? p_at[j] + static_cast<int64_t>(step) * kDepth *
-                                            a.p_row
-                            : zeros;
+          int const row = p_row(j);
+          if constexpr (kWGrad) {
+            g = p_at[j] +
+                static_cast<int64_t>(slots[step & 3][row]) * a.p_row;
+          } else {
+            g = p_at[j];
+            p_at[j] += kDepth * a.p_row;
+          }
+          g = step * kDepth + row < depth ? g : zeros;
         }
-        lds_load16(g, base + (wave * kPLoads + j) * 1024);
+        lds_load16<j * 1024>(on, g, my_p + buf);
       }
+    } else {
+      constexpr int k = j - kPLoads;
+      char const* g;
+      if constexpr (!kQTurned) {
+        g = k8 || step * kStep + q_chunk(k) * 16 < depth * kSize ? q_at[k]
+                                                                : zeros;
+        q_at[k] += kStep;
+      } else {
+        int const row = q_row(k);
+        g = q_at[k] + static_cast<int64_t>(slots[step & 3][row]) * a.q_row;
+        g = step * kDepth + row < depth ? g : zeros;
+      }
+      lds_load16<(k / kHalf) * (kQBytes / 2) + (k % kHalf) * 1024>(
+          on, g, my_q + buf);
+    }
+  };
+  // A step's scales, 4 steps in a ring: the first BQ / 64 waves load those of
+  // Q, the next one those of the tile's blocks of P.
+  static_assert(!k8 || BQ / 64 < kWaves, "a wave for the scales of P");
+  uint32_t const my_s =
+      wave < BQ / 64 ? lds_addr(q_scale) + wave * 256 : lds_addr(p_scale);
+  uint32_t const s_pitch = wave < BQ / 64 ? BQ * 4 : 256;
+  auto load_scales = [&](int on, int step) __attribute__((always_inline)) {
+    if constexpr (k8) {
+      lds_load4(on & before(wave, BQ / 64 + 1), scale_at,
+                uniform(my_s + (step & 3) * s_pitch));
+      scale_at += 4;
+    }
+  };
+  // Weight gradient: the first wave notes the slots of a stage's rows.
+  int seg = 0, seg_begin = 0, seg_end = 0;
+  auto note_slots = [&](Tile const& t, int step) {
+    if constexpr (kWGrad) {
+      if (threadIdx.x < kDepth) {
+        int const i = step * kDepth + threadIdx.x;
+        if (step == 0) {
+          seg = 0;
+          seg_begin = 0;
+          seg_end = table.end[t.e * a.rows.sources];
+        }
+        if (i < t.valid) {
+          while (i >= seg_end) {  // ends: the last end is t.valid
+            ++seg;
+            seg_begin = seg_end;
+            seg_end = table.end[t.e * a.rows.sources + seg];
+          }
+          slots[step & 3][threadIdx.x] =
+              seg * a.rows.length + i - seg_begin;
+        }
+      }
+    }
+  };
+  auto note_rows = [&](Tile const& t, int turn) {
+    if constexpr (!kWGrad)
+      for (int j = threadIdx.x; j < BQ; j += kThreads)
+        slots[turn][j] =
+            slot_of(table, a.rows, t.e, min(t.q0 + j, t.valid - 1));
+  };
+  // The first two stages of a tile whose rows are noted.
+  auto begin_tile = [&](Tile const& t, int turn) {
+    if constexpr (kWGrad) {
+      note_slots(t, 0);
+      note_slots(t, 1);
+    }
+    // slots are noted, and nobody reads the stages any more
+    stage_barrier<kLoads, kLoads + kStores>(0);
+    set_tile(t, turn);
 #pragma unroll
-      for (int j = 0; j < kQLoads; ++j) {
-        int const at = (wave * kQLoads + j) * 64 + lane;
-        char const* g;
-        if constexpr (!kQTurned) {
-          int const c = (at & 7) ^ ((at >> 3) & 7);
-          int const left = a.depth * kSize - step * kStep - c * 16;
-          g = left > 0 ? q_at[j] + static_cast<int64_t>(step) * kStep : zeros;
-        } else {
-          int const row = step * kDepth + at / (BQ / 8);
-          g = row < depth
-                  ? q_at[j] + static_cast<int64_t>(
-                                  slots[(step & 1) * kDepth + at / (BQ / 8)]) *
-                                  a.q_row
-                  : zeros;
-        }
-        lds_load16(g, base + kPBytes + (wave * kQLoads + j) * 1024);
-      }
-      if constexpr (k8)
-        lds_load4(s_at + static_cast<int64_t>(step) * 4,
-                  base + kPBytes + kQBytes + (wave % (BQ / 64)) * 256);
-    };
+    for (int step = 0; step < 2; ++step) {
+      int const on = before(step, steps);
+      unrolled<0, kFirst>([&](auto n) { load_part(n, on, step); });
+      load_scales(on, step);
+      unrolled<kFirst, kLoads>([&](auto n) { load_part(n, on, step); });
+    }
+  };
 
-    // --- the product -------------------------------------------------------
+  // --- this lane's part of the LDS reads -----------------------------------
+  // direct: chunks l / 16 and 4 + l / 16 of its row; turned: see turned()
+  uint32_t p_lo, p_hi, q_lo, q_hi;
+  {
+    int const m = lane & 15, g = lane >> 4, r = (lane >> 2) & 3;
+    if constexpr (!kPTurned) {
+      int const row = wp * RP + (m >> 2) * 8 + (m & 3);
+      int const f = ((row >> 1) & 1) | (((row >> 3) & 3) << 1);
+      p_lo = lds0 + row * kStep + ((g ^ f) * 16);
+      p_hi = lds0 + row * kStep + (((4 + g) ^ f) * 16);
+    } else {
+      int const c = wp * (RP / 8) + (lane & 3);
+      p_lo = lds0 + (g * 8 + r) * kPPitch + ((c ^ (r << 2)) * 16);
+      p_hi = lds0 + (g * 8 + r) * kPPitch + (((c + 4) ^ (r << 2)) * 16);
+    }
+    uint32_t const q = lds0 + kPBytes;
+    if constexpr (!kQTurned) {
+      int const row = wq * (RQ / 2) + m;
+      int const f = (row >> 1) & 7;
+      q_lo = q + row * kStep + ((g ^ f) * 16);
+      q_hi = q + row * kStep + (((4 + g) ^ f) * 16);
+    } else {
+      constexpr int kMask = kQPitch / 16 - 1;
+      int const c = wq * (RQ / 16) + (lane & 3);
+      q_lo = q + (g * 8 + r) * kQPitch + ((c ^ ((r << 2) & kMask)) * 16);
+      q_hi = q + (g * 8 + r) * kQPitch + (((c + 4) ^ ((r << 2) & kMask)) * 16);
+    }
+  }
+  auto direct = [](uint32_t lo, uint32_t hi) {
+    i32x4 const x = lds_read<i32x4>(lo), y = lds_read<i32x4>(hi);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // 16 columns of a turned operand: 64 elements of the contraction, 8 of each
+  // half for a lane
+  auto turned = [](uint32_t at, int pitch) {
+    i16x4 const v0 = lds_read_turned(at);
+    i16x4 const v1 = lds_read_turned(at + 4 * pitch);
+    i16x4 const v2 = lds_read_turned(at + 32 * pitch);
+    i16x4 const v3 = lds_read_turned(at + 36 * pitch);
+    i32x4 const x = __builtin_bit_cast(
+        i32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+    i32x4 const y = __builtin_bit_cast(
+        i32x4, __builtin_shufflevector(v2, v3, 0, 1, 2, 3, 4, 5, 6, 7));
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+
+  i32x8 pf[TP], qf[2];
+  float s[2];
+  uint32_t const s_at = lds_addr(q_scale) + (wq * RQ + (lane & 15)) * 4;
+  auto read_p = [&](int step, int i) __attribute__((always_inline)) {
+    uint32_t const buf = (step & 1) * kStage;
+    if constexpr (!kPTurned) {
+      uint32_t const at = buf + ((i >> 1) * 32 + (i & 1) * 4) * kStep;
+      pf[i] = direct(p_lo + at, p_hi + at);
+    } else {
+      pf[i] = turned((i >> 1 ? p_hi : p_lo) + buf + (i & 1) * 8, kPPitch);
+    }
+  };
+  auto read_q = [&](int step, int j) __attribute__((always_inline)) {
+    uint32_t const buf = (step & 1) * kStage + (j >= TQ / 2) * (kQBytes / 2);
+    int const i = j % (TQ / 2);
+    if constexpr (!kQTurned) {
+      qf[j & 1] = direct(q_lo + buf + i * 16 * kStep,
+                         q_hi + buf + i * 16 * kStep);
+    } else {
+      qf[j & 1] = turned((i >> 1 ? q_hi : q_lo) + buf + (i & 1) * 8, kQPitch);
+    }
+  };
+  auto read_s = [&](int step, int j) __attribute__((always_inline)) {
+    if constexpr (k8)
+      s[j & 1] = lds_read<float>(s_at + (step & 3) * (BQ * 4) + j * 64);
+  };
+
+  Tile now = find_tile<kMode, BP, BQ>(a, table, tile, tiles_p);
+  note_rows(now, 0);
+  begin_tile(now, 0);
+  // What may be in flight behind the loads that a barrier waits for: a stage's
+  // loads, and for the first step and a half of a tile the stores of a whole
+  // tile before it.
+  int left = kLoads;
+  for (int turn = 0;;) {
     f32x4 acc[TP][TQ];
 #pragma unroll
-    for (int i2 = 0; i2 < TP; ++i2)
+    for (int i = 0; i < TP; ++i)
 #pragma unroll
-      for (int j = 0; j < TQ; ++j) acc[i2][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < TQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    float const* p_scale = nullptr;
-    if constexpr (k8) {
-      int const block =
-          min(p0 + wp * (BP / WP), a.np - 1) / 128;  // uniform in a wave
-      p_scale = reinterpret_cast<float const*>(
-          a.p_scales + e * a.ps_expert + block * a.ps_row);
+    // The next tile is looked up while the first stage is on its way.
+    Tile const done = now;
+    int const next_turn = turn < 2 ? turn + 1 : 0;
+    tile += gridDim.x;
+    bool const more = tile < total;
+    if (more) {
+      now = find_tile<kMode, BP, BQ>(a, table, tile, tiles_p);
+      note_rows(now, next_turn);
     }
-
-    // Operand fragment of 16 rows (or columns) from `row0`: 16 bits, the
-    // 32 contraction elements of half `h`; lane l has row l % 16, elements
-    // (l / 16) * 8 on. Both operands use the same order of the contraction.
-    auto direct16 = [&](char const* tile_at, int row0, int h) {
-      int const row = row0 + (lane & 15);
-      int const c = (h * 4 + (lane >> 4)) ^ (row & 7);
-      return *reinterpret_cast<i32x4 const*>(tile_at + row * kStep + c * 16);
-    };
-    auto turned16 = [&](char const* tile_at, int width, int col0, int h) {
-      i16x4 v[2];
+    // Behind the first stage's loads: the second's, and the last tile's stores.
+    stage_barrier<kLoads, kLoads + kStores>(before(1, steps) & left);
+    read_q(0, 0);
+    read_s(0, 0);
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        int const row = h * 32 + (lane >> 4) * 8 + g * 4 + ((lane >> 2) & 3);
-        int const col = col0 + (lane & 3) * 4;
-        int const c = (col >> 3) ^ turn(row);
-        v[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) i16x4*)(
-                tile_at + row * width * 2 + c * 16 + (col & 7) * 2));
-      }
-      i16x8 const both = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5,
-                                                 6, 7);
-      return __builtin_bit_cast(i32x4, both);
-    };
-    auto direct8 = [&](char const* tile_at, int row0) {
-      int const row = row0 + (lane & 15);
-      int const c = (lane >> 4) * 2;
-      i32x4 const lo = *reinterpret_cast<i32x4 const*>(
-          tile_at + row * kStep + ((c ^ (row & 7)) * 16));
-      i32x4 const hi = *reinterpret_cast<i32x4 const*>(
-          tile_at + row * kStep + (((c + 1) ^ (row & 7)) * 16));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
+    for (int i = 0; i < TP; ++i) read_p(0, i);
+    f32x4 d[4];
+    d[2] = d[3] = f32x4{0.f, 0.f, 0.f, 0.f};
+    s[1] = 0.f;
 
-    if (steps > 0) load_stage(0);
     for (int step = 0; step < steps; ++step) {
-      if constexpr (kWGrad) {
-        // slots of the next stage, behind the same barrier as its loads
-        int const next = (step + 1) * kDepth + static_cast<int>(threadIdx.x);
-        if (threadIdx.x < kDepth && next < depth)
-          slots[((step + 1) & 1) * kDepth + threadIdx.x] =
-              slot_of(a.rows, e, next);
-      }
-      stage_barrier();
-      if (step + 1 < steps) load_stage(step + 1);
-      char const* const pt = stages + (step & 1) * kStage;
-      char const* const qt = pt + kPBytes;
-      if constexpr (k8) {
-        float const sw = p_scale[step];
-        float const* const sx = reinterpret_cast<float const*>(qt + kQBytes);
-        i32x8 pf[TP];
+      float sw = 0.f;
+      if constexpr (k8)
+        sw = lds_read<float>(lds_addr(p_scale) + (step & 3) * 256 +
+                             wp * RP / 128 * 4);
+      int const on = before(step + 2, steps);
+      if constexpr (kWGrad)
+        if (on) note_slots(done, step + 2);
+      // Twice in a step, when all waves have read what lies in P and the
+      // first half of Q, and in the second, the loads of the stage after
+      // next take their places; so loads have a step and a half to land.
+      constexpr int kMid = (TQ / 2 - 1) * TP, kEnd = (TQ - 1) * TP;
+      unrolled<0, kT>([&](auto at) __attribute__((always_inline)) {
+        constexpr int t = decltype(at)::value, j = t / TP, i = t % TP;
+        if constexpr (t == kMid || t == kEnd)
+          stage_barrier<kLoads, kLoads + kStores>(on & left);
+        if constexpr (t == kMid)
+          if (step == 1) left = kLoads;
+        if constexpr (k8) {
+          // 8 bits: each product of a block of 128 is added, scaled, while
+          // the next one is in the matrix unit
+          constexpr int last = (t + kT - 2) % kT, jl = last / TP,
+                        il = last % TP;
+          d[t & 3] = mfma8(pf[i], qf[j & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (i == 1) s[j & 1] *= sw;
 #pragma unroll
-        for (int i2 = 0; i2 < TP; ++i2)
-          pf[i2] = direct8(pt, wp * (BP / WP) + i2 * 16);
-#pragma unroll
-        for (int j = 0; j < TQ; ++j) {
-          int const row = wq * (BQ / WQ) + j * 16;
-          i32x8 const qf = direct8(qt, row);
-          float const s = sx[row + (lane & 15)] * sw;
-#pragma unroll
-          for (int i2 = 0; i2 < TP; ++i2) {
-            f32x4 const d = mfma8(pf[i2], qf);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              acc[i2][j][r] = fmaf(d[r], s, acc[i2][j][r]);
+          for (int r = 0; r < 4; ++r)
+            acc[il][jl][r] = fmaf(d[last & 3][r], s[jl & 1], acc[il][jl][r]);
+          // keeps the order of products and sums; a real instruction, as
+          // the compiler counts it as one
+          asm volatile("s_nop 0" ::"v"(acc[il][jl][0]), "v"(acc[il][jl][1]),
+                       "v"(acc[il][jl][2]), "v"(acc[il][jl][3]));
+        } else {
+          // 16 bits: a stage is two products deep, the first for all tiles
+          // of a column, then the second
+          constexpr int h = i / 2;
+          unrolled<0, 2>([&](auto o) __attribute__((always_inline)) {
+            constexpr int ii = i % 2 * 2 + decltype(o)::value;
+            acc[ii][j] = mfma16<kElem>(half<h>(pf[ii]), half<h>(qf[j & 1]),
+                                       acc[ii][j]);
+          });
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (i == 0) read_q(step + (j + 1) / TQ, (j + 1) % TQ);
+        if constexpr (i == 1) read_s(step + (j + 1) / TQ, (j + 1) % TQ);
+        if constexpr (k8) {
+          if constexpr (j == TQ - 1) read_p(step + 1, i);
+        } else {
+          if constexpr (j == TQ - 1 && i >= 2) {
+            read_p(step + 1, i * 2 - 4);
+            read_p(step + 1, i * 2 - 3);
           }
         }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          i32x4 pf[TP];
-#pragma unroll
-          for (int i2 = 0; i2 < TP; ++i2) {
-            int const at = wp * (BP / WP) + i2 * 16;
-            pf[i2] = kPTurned ? turned16(pt, BP, at, h) : direct16(pt, at, h);
-          }
-#pragma unroll
-          for (int j = 0; j < TQ; ++j) {
-            int const at = wq * (BQ / WQ) + j * 16;
-            i32x4 const qf =
-                kQTurned ? turned16(qt, BQ, at, h) : direct16(qt, at, h);
-#pragma unroll
-            for (int i2 = 0; i2 < TP; ++i2)
-              acc[i2][j] = mfma16<kElem>(pf[i2], qf, acc[i2][j]);
-          }
+        if constexpr (t >= kMid && t < kEnd) {
+          constexpr int u = (t - kMid) * 2, kU = kEnd - kMid;  // early
+          unrolled<less(u * kFirst / kU, kFirst),
+                   less((u + 2) * kFirst / kU, kFirst)>(
+              [&](auto n) __attribute__((always_inline)) {
+                load_part(n, on, step + 2);
+              });
+          if constexpr (t == kEnd - 1) load_scales(on, step + 2);
+        } else if constexpr (t >= kEnd) {
+          constexpr int u = t - kEnd;
+          unrolled<kFirst + u * kHalf / TP, kFirst + (u + 1) * kHalf / TP>(
+              [&](auto n) __attribute__((always_inline)) {
+                load_part(n, on, step + 2);
+              });
         }
-      }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    }
+    if constexpr (k8) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[TP - 2][TQ - 1][r] =
+            fmaf(d[2][r], s[1], acc[TP - 2][TQ - 1][r]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[TP - 1][TQ - 1][r] =
+            fmaf(d[3][r], s[1], acc[TP - 1][TQ - 1][r]);
     }
 
-    // --- results -----------------------------------------------------------
-    constexpr int kOutSize = kOut == Elem::kF32 ? 4 : 2;
-    bool const wide = a.np % 4 == 0 && a.out_row % (4 * kOutSize) == 0 &&
-                      a.out_expert % (4 * kOutSize) == 0 &&
-                      reinterpret_cast<uintptr_t>(a.out) % (4 * kOutSize) == 0;
-    int const end_q = kWGrad ? a.nq : valid;
+    // The next tile's first loads go out before this one's results.
+    if (more) begin_tile(now, next_turn);
+    char* const out = a.out + done.e * a.out_expert +
+                      static_cast<int64_t>(done.p0 + wp * RP + (lane >> 4) * 8) *
+                          kOutSize;
+    auto row_of = [&](int j) {
+      if constexpr (!kQTurned)
+        return wq * RQ + j * 16 + (lane & 15);
+      else
+        return wq * RQ + (j >> 1) * 32 + ((lane & 15) >> 2) * 8 +
+               (j & 1) * 4 + (lane & 3);
+    };
+    if (a.wide && done.p0 + BP <= a.np) {
+      // All columns are inside, and a row behind the last holds what a row
+      // inside does, which it stores again: so every lane stores, and the
+      // number of stores in flight is known.
+      left = kLoads + kStores;
 #pragma unroll
-    for (int j = 0; j < TQ; ++j) {
-      int const in_q = wq * (BQ / WQ) + j * 16 + (lane & 15);
-      if (q0 + in_q >= end_q) continue;
-      int64_t const row = kWGrad ? q0 + in_q : slots[in_q];
-      char* const o = a.out + e * a.out_expert + row * a.out_row;
+      for (int j = 0; j < TQ; ++j) {
+        int64_t row;
+        if constexpr (kWGrad) {
+          int const q = done.q0 + row_of(j);
+          row = q < a.nq ? q : a.nq - 8 + (q & 7);
+        } else {
+          row = slots[turn][row_of(j)];
+        }
+        char* const o = out + row * a.out_row;
 #pragma unroll
-      for (int i2 = 0; i2 < TP; ++i2) {
-        int const p = p0 + wp * (BP / WP) + i2 * 16 + (lane >> 4) * 4;
-        if (p < a.np)
-          store4<kOut>(o + static_cast<int64_t>(p) * kOutSize, acc[i2][j],
-                       a.np - p, wide);
+        for (int i = 0; i < TP; i += 2)
+          store8<kOut>(o + i * 16 * kOutSize, acc[i][j], acc[i + 1][j]);
+      }
+    } else {
+      left = kLoads;
+      int const end_q = kWGrad ? a.nq : done.valid;
+#pragma unroll
+      for (int j = 0; j < TQ; ++j) {
+        if (done.q0 + row_of(j) >= end_q) continue;
+        int64_t const row =
+            kWGrad ? done.q0 + row_of(j) : slots[turn][row_of(j)];
+        char* const o = out + row * a.out_row;
+#pragma unroll
+        for (int i = 0; i < TP; i += 2) {
+          int const n = a.np - (done.p0 + wp * RP + (lane >> 4) * 8 + i * 16);
+          if (n >= 8 && a.wide)
+            store8<kOut>(o + i * 16 * kOutSize, acc[i][j], acc[i + 1][j]);
+          else
+            store_few<kOut>(o + i * 16 * kOutSize, acc[i][j], acc[i + 1][j],
+                            n);
+        }
       }
     }
+    if (!more) break;
+    turn = next_turn;
   }
 }
 
@@ -487,6 +809,11 @@ int compute_units() {
   UCCL_CHECK_HIP(
       hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
   return n;
+}
+
+bool stores_wide(GemmArgs const& a) {
+  return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row % 16 == 0 &&
+         a.out_expert % 16 == 0;
 }
 
 template <Mode kMode, Elem kElem, Elem kOut, int BP, int BQ, int WP, int WQ>
@@ -539,6 +866,7 @@ void launch_expert_matmul(MatmulArgs const& m, hipStream_t s) {
   a.out_expert = m.out.expert_stride * out_size;
   a.out_row = m.out.row_stride * out_size;
   a.np = m.n;
+  a.wide = stores_wide(a);
   a.depth = m.k;
   if (m.elem == Elem::kF8) {
     a.p_scales = static_cast<char const*>(m.w_scales.p);
@@ -577,6 +905,7 @@ void launch_expert_weight_grad(WeightGradArgs const& w, hipStream_t s) {
   a.out_expert = w.out.expert_stride * out_size;
   a.out_row = w.out.row_stride * out_size;
   a.np = w.k;
+  a.wide = stores_wide(a);
   a.nq = w.n;
   if (w.elem == Elem::kBF16)
     by_out<Mode::kWeightGrad, Elem::kBF16>(a, w.out_elem, w.n, s);

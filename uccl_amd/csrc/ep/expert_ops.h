@@ -16,7 +16,8 @@ enum class Elem : int { kF8 = 0, kBF16 = 1, kF16 = 2, kF32 = 3 };
 constexpr int kMaxRouteExperts = 1024;  // a wave holds a row, 16 a lane
 constexpr int kMaxRouteTopk = 64;       // one lane for each pick
 constexpr int kMaxRouteGroups = 64;     // one bit of a lane mask each
-constexpr int kMaxSlotExperts = 1024;   // tile prefix held in LDS
+constexpr int kMaxSlotExperts = 1024;   // experts, and experts * sources:
+constexpr int kMaxSlotCells = 2048;     // their row counts are held in LDS
 
 // Rows of a slot array [experts, sources * length, cols]: source r of
 // expert e has counts[e * sources + r] valid rows from r * length on.

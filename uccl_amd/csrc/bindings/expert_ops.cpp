@@ -410,7 +410,7 @@ void expert_swiglu(at::Tensor h, OptTensor counts, at::Tensor out,
   a.rows = rows_of(h, counts);
   a.h = mat_of(h, "h");
   a.cols = static_cast<int>(cols);
-  TORCH_CHECK(h.size(2) < (int64_t(1) << 31), "uccl_amd: too many columns");
+  TORCH_CHECK(h.size(2) < (int64_t(1) << 24), "uccl_amd: too many columns");
   a.elem = elem_of(h, "h");
   a.quantize = scales.has_value();
   std::vector<at::Tensor> operands{h};
@@ -451,7 +451,7 @@ void expert_swiglu_grad(at::Tensor grad, at::Tensor h, OptTensor counts,
   TORCH_CHECK(cols >= 8 && h.size(2) % 16 == 0,
               "uccl_amd: h has two halves of a multiple of 8 columns, got ",
               h.size(2));
-  TORCH_CHECK(h.size(2) < (int64_t(1) << 31), "uccl_amd: too many columns");
+  TORCH_CHECK(h.size(2) < (int64_t(1) << 24), "uccl_amd: too many columns");
   TORCH_CHECK(grad.scalar_type() == h.scalar_type() &&
                   out.scalar_type() == h.scalar_type(),
               "uccl_amd: grad_out and out must have the dtype of h");

@@ -5,142 +5,471 @@
 //              q = the e4m3 value nearest to v / s, ties to even
 //   gradient: da = g b sig(a) (1 + a (1 - sig(a))), db = g silu(a)
 //
-// Bound by memory: every value is read and written once, 16 bytes a lane.
+// Bound by memory: every value is read and written once, 16 bytes a lane and
+// load. A wave takes 512 columns of a row, or several rows of fewer columns.
+//
+// The exponential is taken of -|a| / 2 and used twice, w = exp(-|a| / 2): for
+// a < 0 sig(a) = w w / (1 + w w), and the factors of a product take one w
+// each, so nothing overflows and no product of normal size is lost to an
+// underflow on the way.
+//
+// 8 bits: scales and values are those of exact arithmetic, whatever the last
+// bits of a float exponential are. Only the largest |v| of a group is worked
+// out in 64 bits, and values that lie so close to the middle between two 8-bit
+// values that 32 bits do not decide; groups outside 1e-30 .. 1e30 entirely.
 
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
-#include "../core/log.h"
-#include "../device/primitives.h"
 #include "expert_ops.h"
 
 namespace uccl {
 namespace ep {
 
-using namespace uccl::device;
-
 namespace {
 
-__device__ __forceinline__ int clamp_count(SlotRows const& r, int i) {
-  return r.counts ? min(max(r.counts[i], 0), r.length) : r.length;
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <typename T>
+using x8 = T __attribute__((ext_vector_type(8)));
+
+constexpr int kUnit = 8;  // columns of a lane
+
+// How a wave's lanes lie on the rows of a cell: 64 lanes on 512 columns of a
+// row, or several rows of fewer columns.
+struct Part {
+  int rows;   // rows that a wave takes together
+  int lanes;  // lanes of a row
+  int parts;  // waves' shares of a row
+};
+
+__host__ __device__ inline Part part_of(int cols) {
+  int const units = cols / kUnit;
+  if (units < 64) return {64 / units, units, 1};
+  return {1, 64, (units + 63) / 64};
 }
 
-__device__ __forceinline__ double silu_mul(double a, double b) {
-  return a / (1.0 + exp(-a)) * b;
+struct Share {
+  int at;   // row of the cell
+  int col;  // first column
+  bool on;  // whether the lane has work
+};
+
+// Takes this wave through its shares of the cell's valid rows, kShares at a
+// time: parts of a row next to each other, or rows where a row is one share.
+// load(shares) asks for a turn's data while work(shares, data) is at the turn
+// before. blockIdx: cell, rows, parts. All lanes of a wave call both together.
+template <int kShares, bool kSplit, typename Load, typename Work>
+__device__ __forceinline__ void each_share(SlotRows const& r, int cols,
+                                           Load&& load, Work&& work) {
+  Part const p = kSplit ? Part{1, 64, 0} : part_of(cols);
+  int const lane = threadIdx.x & 63;
+  int const cell = blockIdx.x;
+  int const valid =
+      r.counts ? min(max(r.counts[cell], 0), r.length) : r.length;
+  int const row = kSplit ? 0 : lane / p.lanes;
+  int const in_row = lane - row * p.lanes;
+  int const waves = gridDim.y * (blockDim.x >> 6);
+  int const part = kSplit ? blockIdx.z * kShares : 0;
+  int64_t const stride = static_cast<int64_t>(waves) * p.rows;
+  int64_t const turn = kSplit ? stride : stride * kShares;
+  struct Shares {
+    Share s[kShares];
+  };
+  auto shares_at = [&](int64_t first) {
+    Shares t;
+#pragma unroll
+    for (int k = 0; k < kShares; ++k) {
+      int64_t const begin = first + (kSplit ? 0 : k * stride) + row;
+      t.s[k].at = begin < valid ? static_cast<int>(begin) : valid;
+      t.s[k].col = ((part + (kSplit ? k : 0)) * 64 + in_row) * kUnit;
+      t.s[k].on = row < p.rows && t.s[k].at < valid && t.s[k].col < cols;
+    }
+    return t;
+  };
+  int64_t first = (blockIdx.y * static_cast<int64_t>(blockDim.x >> 6) +
+                   __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) *
+                  p.rows;
+  if (first >= valid) return;
+  Shares now = shares_at(first);
+  auto data = load(now.s);
+  for (;;) {
+    first += turn;
+    Shares const next = shares_at(first);
+    auto const more = load(next.s);
+    work(now.s, data);
+    if (first >= valid) break;
+    now = next;
+    data = more;
+  }
+}
+
+// First row of the block's cell.
+__device__ __forceinline__ char* cell_of(Mat const& m, SlotRows const& r,
+                                         int size) {
+  int const e = blockIdx.x / r.sources;
+  int const source = blockIdx.x - e * r.sources;
+  return static_cast<char*>(m.p) +
+         (e * m.expert_stride +
+          static_cast<int64_t>(source) * r.length * m.row_stride) *
+             size;
+}
+__device__ __forceinline__ char* row_at(char* cell, Mat const& m, int at,
+                                        int size) {
+  return cell + static_cast<int64_t>(at) * m.row_stride * size;
+}
+
+template <typename T>
+__device__ __forceinline__ x8<T> load8(char const* row, int col) {
+  return reinterpret_cast<x8<T> const*>(row)[col / kUnit];
+}
+template <typename T>
+__device__ __forceinline__ f32x8 floats(x8<T> v) {
+  return __builtin_convertvector(v, f32x8);
+}
+template <typename T>
+__device__ __forceinline__ void store8(char* row, int col, f32x8 v) {
+  reinterpret_cast<x8<T>*>(row)[col / kUnit] =
+      __builtin_convertvector(v, x8<T>);
+}
+
+// exp(-|a| / 2), good to about a unit in the last place: the part of the
+// exponent that its product lost is put back.
+__device__ __forceinline__ float half_exp(float a) {
+  // log2(e) / 2, in two parts
+  constexpr float kHigh = 0.72134752f, kLow = 9.629815e-9f;
+  float const x = -fabsf(a);
+  float const h = x * kHigh;
+  float const l = fmaf(x, kLow, fmaf(x, kHigh, -h));
+  float const e = __builtin_amdgcn_exp2f(h);
+  return fmaf(e, l * 0.69314718f, e);
+}
+
+struct Gate {
+  float w;     // 1, or exp(a / 2) where a < 0
+  float norm;  // 1 / (1 + exp(-|a|)); sig(a) = w w norm
+};
+__device__ __forceinline__ Gate gate_of(float a) {
+  float const e = half_exp(a);
+  return {a < 0.f ? e : 1.f, __builtin_amdgcn_rcpf(fmaf(e, e, 1.f))};
+}
+
+__device__ __forceinline__ float silu_mul(float a, float b) {
+  Gate const g = gate_of(a);
+  return (a * g.w) * g.norm * (g.w * b);
+}
+
+__device__ __forceinline__ double silu_mul_exact(float a, float b) {
+  double const x = a;
+  return x / (1.0 + exp(-x)) * static_cast<double>(b);
+}
+
+// Nearest 8-bit value to y, given back as a float, ties to even.
+__device__ __forceinline__ float nearest_exact(double y) {
+  int e;
+  (void)frexp(y, &e);
+  double const step = ldexp(1.0, max(e - 4, -9));
+  double const r = rint(y / step) * step;
+  return static_cast<float>(r > 448.0 ? 448.0 : r < -448.0 ? -448.0 : r);
+}
+
+// Largest of the 16 lanes of a group, in all of them: rotations in a DPP row.
+template <int kBy>
+__device__ __forceinline__ int rotated(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x120 + kBy, 0xf, 0xf, false);
+}
+template <int kBy = 8>
+__device__ __forceinline__ float group_max(float v) {
+  v = fmaxf(v, __builtin_bit_cast(
+                   float, rotated<kBy>(__builtin_bit_cast(int, v))));
+  if constexpr (kBy > 1) v = group_max<kBy / 2>(v);
+  return v;
+}
+template <int kBy = 8>
+__device__ __forceinline__ double group_max(double v) {
+  int2 const w = __builtin_bit_cast(int2, v);
+  v = fmax(v, __builtin_bit_cast(
+                  double, make_int2(rotated<kBy>(w.x), rotated<kBy>(w.y))));
+  if constexpr (kBy > 1) v = group_max<kBy / 2>(v);
+  return v;
+}
+
+// The j-th of 16 values, of two lots of 8.
+template <typename T>
+__device__ __forceinline__ float pick(x8<T> const (&v)[2], int j) {
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
+  i32x4 const p = __builtin_bit_cast(i32x4, v[0]),
+              q = __builtin_bit_cast(i32x4, v[1]);
+  int r = p[0];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) r = (j >> 1) == k ? (k < 4 ? p[k] : q[k - 4]) : r;
+  auto const half =
+      static_cast<unsigned short>(static_cast<unsigned>(r) >> (j & 1) * 16);
+  return static_cast<float>(__builtin_bit_cast(T, half));
 }
 
 }  // namespace
 
-// Grid: (cells = experts * sources, row chunks). One wave takes a row at a
-// time.
-template <typename T, bool kQuantize>
+template <typename T, bool kSplit>
 __global__ __launch_bounds__(256) void k_swiglu(SwigluArgs a) {
-  int const wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int const cell = blockIdx.x;
-  int const e = cell / a.rows.sources, src = cell % a.rows.sources;
-  int const valid = clamp_count(a.rows, cell);
-  for (int i = blockIdx.y * 4 + wave; i < valid; i += gridDim.y * 4) {
-    int64_t const slot = static_cast<int64_t>(src) * a.rows.length + i;
-    T const* row = static_cast<T const*>(a.h.p) + e * a.h.expert_stride +
-                   slot * a.h.row_stride;
-    if constexpr (kQuantize) {
-      __hip_fp8_e4m3* out = static_cast<__hip_fp8_e4m3*>(a.out.p) +
-                            e * a.out.expert_stride + slot * a.out.row_stride;
-      float* scales = static_cast<float*>(a.scales.p) +
-                      e * a.scales.expert_stride + slot * a.scales.row_stride;
-      for (int g = 0; g < a.cols / 128; ++g) {
-        double v[2];
-        double most = 0.0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          int const c = g * 128 + lane * 2 + j;
-          v[j] = silu_mul(static_cast<float>(row[c]),
-                          static_cast<float>(row[a.cols + c]));
-          most = fmax(most, fabs(v[j]));
-        }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1)
-          most = fmax(most, __shfl_xor(most, off));
-        float const scale = most > 0.0 ? static_cast<float>(most / 448.0) : 1.f;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          double const y = v[j] / scale;
-          int ex;
-          frexp(y, &ex);
-          double const step = ldexp(1.0, max(ex - 4, -9));
-          out[g * 128 + lane * 2 + j] =
-              __hip_fp8_e4m3(static_cast<float>(rint(y / step) * step));
-        }
-        if (lane == 0) scales[g] = scale;
-      }
-    } else {
-      T* out = static_cast<T*>(a.out.p) + e * a.out.expert_stride +
-               slot * a.out.row_stride;
-      for (int c = lane; c < a.cols; c += 64) {
-        float const x = static_cast<float>(row[c]);
-        float const b = static_cast<float>(row[a.cols + c]);
-        out[c] = static_cast<T>(x / (1.f + expf(-x)) * b);
-      }
+  char* const h_cell = cell_of(a.h, a.rows, sizeof(T));
+  char* const out_cell = cell_of(a.out, a.rows, sizeof(T));
+  struct Data {
+    x8<T> x, b;
+  };
+  auto load = [&](Share const (&s)[1]) {
+    Data d{};
+    if (s[0].on) {
+      char const* const h = row_at(h_cell, a.h, s[0].at, sizeof(T));
+      d.x = load8<T>(h, s[0].col);
+      d.b = load8<T>(h, a.cols + s[0].col);
     }
-  }
+    return d;
+  };
+  each_share<1, kSplit>(a.rows, a.cols, load, [&](Share const (&s)[1], Data const& d) {
+    if (!s[0].on) return;
+    f32x8 const x = floats<T>(d.x), b = floats<T>(d.b);
+    f32x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = silu_mul(x[j], b[j]);
+    store8<T>(row_at(out_cell, a.out, s[0].at, sizeof(T)), s[0].col, v);
+  });
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_swiglu_grad(SwigluArgs a) {
-  int const wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int const cell = blockIdx.x;
-  int const e = cell / a.rows.sources, src = cell % a.rows.sources;
-  int const valid = clamp_count(a.rows, cell);
-  for (int i = blockIdx.y * 4 + wave; i < valid; i += gridDim.y * 4) {
-    int64_t const slot = static_cast<int64_t>(src) * a.rows.length + i;
-    T const* row = static_cast<T const*>(a.h.p) + e * a.h.expert_stride +
-                   slot * a.h.row_stride;
-    T const* gr = static_cast<T const*>(a.grad_out.p) +
-                  e * a.grad_out.expert_stride + slot * a.grad_out.row_stride;
-    T* out = static_cast<T*>(a.out.p) + e * a.out.expert_stride +
-             slot * a.out.row_stride;
-    for (int c = lane; c < a.cols; c += 64) {
-      float const x = static_cast<float>(row[c]);
-      float const b = static_cast<float>(row[a.cols + c]);
-      float const g = static_cast<float>(gr[c]);
-      float const sig = 1.f / (1.f + expf(-x));
-      out[c] = static_cast<T>(g * b * sig * (1.f + x * (1.f - sig)));
-      out[a.cols + c] = static_cast<T>(g * x * sig);
+// Two shares at a time, so that one pass in 64 bits serves both: each lane
+// brings the largest of its values, if that may be its group's largest.
+template <typename T, bool kSplit>
+__global__ __launch_bounds__(256) void k_swiglu_quant(SwigluArgs a) {
+  constexpr int kShares = 2;
+  char* const h_cell = cell_of(a.h, a.rows, sizeof(T));
+  char* const out_cell = cell_of(a.out, a.rows, 1);
+  char* const scale_cell = cell_of(a.scales, a.rows, 4);
+  struct Data {
+    x8<T> x[kShares], b[kShares];
+  };
+  auto load = [&](Share const (&s)[kShares]) {
+    Data d{};
+#pragma unroll
+    for (int k = 0; k < kShares; ++k)
+      if (s[k].on) {
+        char const* const h = row_at(h_cell, a.h, s[k].at, sizeof(T));
+        d.x[k] = load8<T>(h, s[k].col);
+        d.b[k] = load8<T>(h, a.cols + s[k].col);
+      }
+    return d;
+  };
+  each_share<kShares, kSplit>(a.rows, a.cols, load, [&](Share const (&s)[kShares],
+                                                Data const& raw) {
+    // a group's 128 columns are 16 neighbouring lanes, all of them on or off
+    f32x8 v[kShares];
+    // v in 32 bits, good to (|a| + 6) 2^-24 of its size: an exponential of a
+    // rounded product and five operations more. Groups with a below -85,
+    // where the exponential ends, or whose largest |v| is far from 1 are
+    // `wild`: nothing of them is decided in 32 bits.
+    bool wild[kShares];
+    float limit[kShares];         // below it, no value is its group's largest
+    float top_x[kShares], top_b[kShares];  // where this lane's largest is
+    unsigned open = 0;  // shares with a lane's largest to work out
+    unsigned left = 0;  // further values, when one does not do
+#pragma unroll
+    for (int k = 0; k < kShares; ++k) {
+      f32x8 const x = floats<T>(raw.x[k]), b = floats<T>(raw.b[k]);
+      float most = -1.f, second = -1.f, lowest = 0.f;
+      top_x[k] = top_b[k] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float const e = __builtin_amdgcn_exp2f(x[j] * -1.44269504f);
+        v[k][j] = x[j] * b[j] * __builtin_amdgcn_rcpf(1.f + e);
+        float const size = fabsf(v[k][j]);
+        bool const more = size > most;
+        top_x[k] = more ? x[j] : top_x[k];
+        top_b[k] = more ? b[j] : top_b[k];
+        second = __builtin_amdgcn_fmed3f(second, size, most);
+        most = fmaxf(most, size);
+        lowest = fminf(lowest, x[j]);
+      }
+      float const group = group_max(lowest < -85.f ? INFINITY : most);
+      wild[k] = !(group >= 1e-20f && group <= 1e30f);
+      limit[k] = group * (1.f - 0x1p-15f);
+      if (s[k].on) {
+        if (!wild[k] && most >= limit[k]) open |= 1u << k;
+        if (wild[k] || second >= limit[k]) left |= 0xffu << (k * 8);
+      }
     }
-  }
+    double exact[kShares] = {};
+    while (open) {
+      int const k = __builtin_ctz(open);
+      open &= open - 1;
+      double const size = fabs(silu_mul_exact(k ? top_x[1] : top_x[0],
+                                              k ? top_b[1] : top_b[0]));
+      exact[0] = fmax(exact[0], k ? 0.0 : size);
+      exact[1] = fmax(exact[1], k ? size : 0.0);
+    }
+    while (left) {
+      int const j = __builtin_ctz(left);
+      left &= left - 1;
+      double const size =
+          fabs(silu_mul_exact(pick<T>(raw.x, j), pick<T>(raw.b, j)));
+      exact[0] = fmax(exact[0], j < 8 ? size : 0.0);
+      exact[1] = fmax(exact[1], j < 8 ? 0.0 : size);
+    }
+    // 20 bits of a float lie behind the 3 of an 8-bit value. Where they are
+    // within kNear of one half, 32 bits do not decide: the error above, and
+    // 2 units of the scaling, are at most 96 of those bits.
+    constexpr unsigned kNear = 112;
+    float scale[kShares];
+    auto behind = [](float y) {
+      float const size = fabsf(y);
+      // below 2^-6 the steps no longer shrink
+      float const fixed = size < 0x1p-6f ? size + 0x1p-6f : size;
+      return (__builtin_bit_cast(unsigned, fixed) + 0x80000u + kNear) &
+             0xfffffu;
+    };
+    unsigned near = 0;
+#pragma unroll
+    for (int k = 0; k < kShares; ++k) {
+      double const largest = group_max(exact[k]);
+      // the quotient by 448, rounded once: a product with 1 / 448, corrected
+      double q = largest * (1.0 / 448.0);
+      q = fma(fma(-448.0, q, largest), 1.0 / 448.0, q);
+      scale[k] =
+          largest > 0.0
+              ? static_cast<float>(largest < INFINITY ? q : largest)
+              : 1.f;
+      float const inverse = __builtin_amdgcn_rcpf(scale[k]);
+      unsigned nearest = ~0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[k][j] *= inverse;
+        nearest = min(nearest, behind(v[k][j]));
+      }
+      if (s[k].on && (nearest <= 2 * kNear || wild[k])) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (behind(v[k][j]) <= 2 * kNear || wild[k])
+            near |= 1u << (k * 8 + j);
+      }
+    }
+    while (near) {
+      int const j = __builtin_ctz(near);
+      near &= near - 1;
+      float const y =
+          nearest_exact(silu_mul_exact(pick<T>(raw.x, j), pick<T>(raw.b, j)) /
+                        (j < 8 ? scale[0] : scale[1]));
+#pragma unroll
+      for (int k = 0; k < kShares; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[k][i] = j == k * 8 + i ? y : v[k][i];
+    }
+#pragma unroll
+    for (int k = 0; k < kShares; ++k) {
+      if (!s[k].on) continue;
+      int lo = 0, hi = 0;
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][0], v[k][1], lo, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][2], v[k][3], lo, true);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][4], v[k][5], hi, false);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][6], v[k][7], hi, true);
+      char* const out = row_at(out_cell, a.out, s[k].at, 1);
+      *reinterpret_cast<int2*>(out + s[k].col) = make_int2(lo, hi);
+      if ((threadIdx.x & 15) == 0)
+        reinterpret_cast<float*>(
+            row_at(scale_cell, a.scales, s[k].at, 4))[s[k].col / 128] =
+            scale[k];
+    }
+  });
+}
+
+template <typename T, bool kSplit>
+__global__ __launch_bounds__(256) void k_swiglu_grad(SwigluArgs a) {
+  char* const h_cell = cell_of(a.h, a.rows, sizeof(T));
+  char* const g_cell = cell_of(a.grad_out, a.rows, sizeof(T));
+  char* const out_cell = cell_of(a.out, a.rows, sizeof(T));
+  struct Data {
+    x8<T> x, b, g;
+  };
+  auto load = [&](Share const (&s)[1]) {
+    Data d{};
+    if (s[0].on) {
+      char const* const h = row_at(h_cell, a.h, s[0].at, sizeof(T));
+      d.x = load8<T>(h, s[0].col);
+      d.b = load8<T>(h, a.cols + s[0].col);
+      d.g = load8<T>(row_at(g_cell, a.grad_out, s[0].at, sizeof(T)),
+                     s[0].col);
+    }
+    return d;
+  };
+  each_share<1, kSplit>(a.rows, a.cols, load, [&](Share const (&s)[1], Data const& d) {
+    if (!s[0].on) return;
+    int const col = s[0].col;
+    f32x8 const x = floats<T>(d.x), b = floats<T>(d.b), g = floats<T>(d.g);
+    f32x8 da, db;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      Gate const t = gate_of(x[j]);
+      float const gn = (g[j] * t.w) * t.norm;
+      float const sig = t.w * t.w * t.norm;
+      db[j] = gn * (t.w * x[j]);
+      da[j] = gn * (t.w * b[j]) * fmaf(x[j], 1.f - sig, 1.f);
+    }
+    char* const out = row_at(out_cell, a.out, s[0].at, sizeof(T));
+    store8<T>(out, col, da);
+    store8<T>(out, a.cols + col, db);
+  });
 }
 
 namespace {
 
-dim3 row_grid(SlotRows const& r) {
-  int const cells = r.experts * r.sources;
-  return dim3(cells, std::max(1, std::min((r.length + 3) / 4, 4096 / cells)));
+// At most kMost blocks, of 4 waves with a row or more each: few enough that
+// a wave has rows to load ahead of, enough to fill the card. The host does not
+// know the counts; a block without rows ends at once.
+constexpr int64_t kMost = 4096;
+dim3 share_grid(SwigluArgs const& a, int shares) {
+  Part const p = part_of(a.cols);
+  int64_t const cells = static_cast<int64_t>(a.rows.experts) * a.rows.sources;
+  int64_t const z = p.parts > 1 ? (p.parts + shares - 1) / shares : 1;
+  int64_t const rows = (a.rows.length + p.rows - 1) / p.rows;
+  int64_t const y = std::min(std::max<int64_t>(1, kMost / (cells * z)),
+                             (rows + 3) / 4);
+  return dim3(static_cast<unsigned>(cells), static_cast<unsigned>(y),
+              static_cast<unsigned>(z));
+}
+
+// f(T{}, whether a row has several shares)
+template <typename F>
+void by_kind(SwigluArgs const& a, F&& f) {
+  auto const split = [&](auto t) {
+    if (part_of(a.cols).parts > 1)
+      f(t, std::true_type{});
+    else
+      f(t, std::false_type{});
+  };
+  if (a.elem == Elem::kBF16)
+    split(__bf16{});
+  else
+    split(_Float16{});
 }
 
 }  // namespace
 
 void launch_expert_swiglu(SwigluArgs const& a, hipStream_t s) {
-  dim3 const grid = row_grid(a.rows);
-  if (a.elem == Elem::kBF16) {
+  dim3 const grid = share_grid(a, a.quantize ? 2 : 1);
+  by_kind(a, [&](auto t, auto split) {
     if (a.quantize)
-      k_swiglu<__hip_bfloat16, true><<<grid, 256, 0, s>>>(a);
+      k_swiglu_quant<decltype(t), decltype(split)::value>
+          <<<grid, 256, 0, s>>>(a);
     else
-      k_swiglu<__hip_bfloat16, false><<<grid, 256, 0, s>>>(a);
-  } else {
-    if (a.quantize)
-      k_swiglu<__half, true><<<grid, 256, 0, s>>>(a);
-    else
-      k_swiglu<__half, false><<<grid, 256, 0, s>>>(a);
-  }
+      k_swiglu<decltype(t), decltype(split)::value><<<grid, 256, 0, s>>>(a);
+  });
 }
 
 void launch_expert_swiglu_grad(SwigluArgs const& a, hipStream_t s) {
-  dim3 const grid = row_grid(a.rows);
-  if (a.elem == Elem::kBF16)
-    k_swiglu_grad<__hip_bfloat16><<<grid, 256, 0, s>>>(a);
-  else
-    k_swiglu_grad<__half><<<grid, 256, 0, s>>>(a);
+  dim3 const grid = share_grid(a, 1);
+  by_kind(a, [&](auto t, auto split) {
+    k_swiglu_grad<decltype(t), decltype(split)::value>
+        <<<grid, 256, 0, s>>>(a);
+  });
 }
 
 }  // namespace ep

@@ -187,6 +187,46 @@ def test_route_strided_and_empty():
     assert torch.equal(idx, idx[:1].expand(5, 4))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("tokens, experts, topk, kw", [
+    (4097, 8, 2, {}),
+    (5000, 64, 6, {}),
+    (4999, 40, 16, dict(scoring="sigmoid", num_groups=5, topk_groups=3)),
+    (4500, 200, 8, dict(bias=1)),
+    (4200, 256, 8, dict(scoring="sigmoid", bias=1, num_groups=8,
+                        topk_groups=4)),
+    (4100, 256, 17, {}),
+    (4100, 300, 5, dict(renormalize=False)),
+])
+def test_route_many_tokens(tokens, experts, topk, kw, dtype):
+    """A token's picks, weights and gradient do not hang on how many others
+    there are (few tokens have more lanes each), nor on where it stands."""
+    g = gen(tokens)
+    x = (randn(g, tokens, experts) * 2).to(dtype)
+    x[torch.rand(tokens, experts, device="cuda", generator=g) < 0.1] = -math.inf
+    x[7] = -math.inf
+    x[11, 3] = math.nan
+    kw = dict(kw)
+    if kw.pop("bias", 0):
+        kw["bias"] = randn(g, experts) * 0.1
+    gw = randn(g, tokens, topk)
+    how = {k: v for k, v in kw.items() if k in ("scoring", "renormalize")}
+    idx, w = ep.route(x, topk, **kw)
+    grad = ep.route_grad(gw, x, idx, **how)
+    for at in range(0, tokens, 1500):
+        part = slice(at, min(at + 1500, tokens))
+        idx_p, w_p = ep.route(x[part], topk, **kw)
+        assert torch.equal(idx[part], idx_p)
+        close(w[part], w_p, w_p.abs() * 2 ** -23)
+        grad_p = ep.route_grad(gw[part], x[part], idx_p, **how)
+        close(grad[part], grad_p, grad_p.abs() * half_step(dtype) * 2 + 1e-13)
+    some = torch.randint(0, tokens, (20,), device="cuda", generator=g)
+    some[:2] = torch.tensor([7, 11], device="cuda")
+    want_idx, want_w = route_oracle(x[some], topk, **kw)
+    assert torch.equal(idx[some].cpu(), want_idx)
+    close(w[some].cpu(), want_w, want_w.abs() * 2 ** -23 + 1e-45)
+
+
 def weights_of(x, idx, scoring, renormalize, scale):
     """The weights as a function of 64-bit logits, the picks held fixed."""
     s = torch.sigmoid(x) if scoring == "sigmoid" else torch.softmax(x, -1)

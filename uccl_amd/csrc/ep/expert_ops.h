@@ -40,6 +40,9 @@ struct RouteArgs {
   int groups, topk_groups, group_best;
   bool renormalize;
   float scale;
+  // set by the launchers: rows can be read, the gradient's be written, a
+  // lane's experts at a time
+  bool whole, whole_out;
 };
 void launch_route(RouteArgs const& a, int64_t* idx, float* weights,
                   hipStream_t s);

@@ -2,26 +2,31 @@
 //
 //   score  s_e = softmax(x)_e or sigmoid(x_e); an expert whose logit is -inf
 //          is closed: it has no score and is never picked
-//   key    s_e + bias_e, or x_e itself without a bias (the same order)
+//   rank   s_e + bias_e, or x_e itself without a bias (the same order)
 //   groups value of a group = sum of its `group_best` largest s_e + bias_e;
 //          only experts of the topk_groups best groups stay
-//   picks  the topk largest keys, ties to the lowest index; a row with fewer
+//   picks  the topk largest ranks, ties to the lowest index; a row with fewer
 //          open experts gets index -1 and weight 0 behind them
 //   weight scale * s_k / sum_j s_j, or scale * s_k
 //
-// Keys are formed and compared in 64 bits: two experts' keys often lie within
-// a few units of the last place of a float, and the choice must not hang on
-// the order in which a float sum was taken. CDNA4 runs 64-bit FMA at the
-// vector rate of 32 bits, so this costs no extra pass over memory.
+// Ranks with a bias or groups are formed and compared in 64 bits: two experts'
+// ranks often lie within a few units of the last place of a float, and the
+// choice must not hang on the order in which a float sum was taken. CDNA4 runs
+// 64-bit FMA at the vector rate of 32 bits, so this costs no extra pass over
+// memory. Without them the logits are compared as they are.
 //
-// A wave holds a token's row in registers, lane l the experts l, l + 64, ...
-// (coalesced loads). A pick is an argmax over the wave: the high word of the
-// order-preserving integer image of the key is maximised with DPP steps, and
-// only when several lanes share it the low word and the index are.
+// A token's row lies in the registers of 64 or 16 lanes, neighbouring experts
+// in a lane. 64 lanes are the shorter way for a token (what counts while the
+// card has idle waves), 16 take a third of the instructions (what counts when
+// it has not): four tokens share a wave, and a maximum over a row of 16 lanes
+// is four DPP rotations. A pick is an argmax over the row: the high word of an
+// order-preserving integer image of the rank is maximised first, the rest only
+// among the lanes that share it.
 
 #include <hip/hip_runtime.h>
 
-#include "../device/primitives.h"
+#include <type_traits>
+
 #include "expert_ops.h"
 
 namespace uccl {
@@ -31,187 +36,310 @@ namespace {
 
 constexpr int kRouteWaves = 4;
 
-template <typename T>
-__device__ inline double load_logit(T const* p) {
-  return static_cast<double>(static_cast<float>(*p));
-}
+// --- reductions over a token's lanes, the result in all of them ------------
 
-// Integer image of a key: larger key, larger image; 0 is "not to be picked"
-// (closed experts, NaN keys). -0 and 0 are one value.
-__device__ inline uint64_t key_image(double k) {
-  if (!(k > -INFINITY)) return 0;
-  k += 0.0;
-  uint64_t const b = __double_as_longlong(k);
-  return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ uint32_t dpp(uint32_t old, uint32_t v) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(static_cast<int>(old), static_cast<int>(v),
+                                  kCtrl, kRows, 0xf, false));
 }
-
-template <int kCtrl>
-__device__ inline uint32_t dpp_max(uint32_t v) {
-  // lanes without a source keep their own value
-  uint32_t const o = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
-      static_cast<int>(v), static_cast<int>(v), kCtrl, 0xf, 0xf, false));
-  return v > o ? v : o;
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ double dpp(double old, double v) {
+  uint2 const o = __builtin_bit_cast(uint2, old),
+              w = __builtin_bit_cast(uint2, v);
+  return __builtin_bit_cast(double, make_uint2(dpp<kCtrl, kRows>(o.x, w.x),
+                                               dpp<kCtrl, kRows>(o.y, w.y)));
 }
-
-// Maximum over the 64 lanes, uniform. Row shifts of 1, 2, 4, 8, then the
-// last lane of a row and of the lower half are broadcast onward.
-__device__ inline uint32_t wave_max(uint32_t v) {
-  v = dpp_max<0x111>(v);
-  v = dpp_max<0x112>(v);
-  v = dpp_max<0x114>(v);
-  v = dpp_max<0x118>(v);
-  v = dpp_max<0x142>(v);
-  v = dpp_max<0x143>(v);
+__device__ __forceinline__ uint32_t lane63(uint32_t v) {
   return static_cast<uint32_t>(
       __builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
-
-__device__ inline double wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  return v;
+__device__ __forceinline__ double lane63(double v) {
+  uint2 const w = __builtin_bit_cast(uint2, v);
+  return __builtin_bit_cast(double, make_uint2(lane63(w.x), lane63(w.y)));
 }
 
-__device__ inline double wave_fmax(double v) {
+// 16 lanes: rotations in a row. 64: shifts by 1, 2, 4, 8 in a row, then the
+// last lane of a row, and of the lower half, is handed on; lanes without a
+// source see `none`.
+template <int kLanes, typename V, typename F>
+__device__ __forceinline__ V over_row(V v, V none, F&& f) {
+  if constexpr (kLanes == 16) {
+    v = f(v, dpp<0x128>(v, v));
+    v = f(v, dpp<0x124>(v, v));
+    v = f(v, dpp<0x122>(v, v));
+    return f(v, dpp<0x121>(v, v));
+  } else {
+    v = f(v, dpp<0x111>(none, v));
+    v = f(v, dpp<0x112>(none, v));
+    v = f(v, dpp<0x114>(none, v));
+    v = f(v, dpp<0x118>(none, v));
+    v = f(v, dpp<0x142, 0xa>(none, v));
+    v = f(v, dpp<0x143, 0xc>(none, v));
+    return lane63(v);
+  }
+}
+template <int kLanes>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  return over_row<kLanes>(v, 0u, [](uint32_t a, uint32_t b) {
+    return a > b ? a : b;
+  });
+}
+template <int kLanes>
+__device__ __forceinline__ double row_max(double v) {
+  return over_row<kLanes>(v, -static_cast<double>(INFINITY),
+                          [](double a, double b) { return fmax(a, b); });
+}
+template <int kLanes>
+__device__ __forceinline__ double row_sum(double v) {
+  return over_row<kLanes>(v, 0.0, [](double a, double b) { return a + b; });
+}
+
+// Integer images of ranks: larger rank, larger image; 0 is "not to be picked"
+// (closed experts, NaN ranks), and every other image has a bit of its high
+// word set. -0 and 0 are one value.
+__device__ __forceinline__ uint64_t image(double k) {
+  if (!(k > -static_cast<double>(INFINITY))) return 0;
+  uint64_t const b = __double_as_longlong(k + 0.0);
+  return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ uint32_t image(float k) {
+  if (!(k > -INFINITY)) return 0;
+  uint32_t const b = __builtin_bit_cast(uint32_t, k + 0.f);
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_image(uint32_t i) {
+  return __builtin_bit_cast(float, (i >> 31) ? i & 0x7fffffffu : ~i);
+}
+
+template <bool kSigmoid>
+__device__ __forceinline__ double score_of(double x, double top,
+                                           double total) {
+  if constexpr (kSigmoid) return 1.0 / (1.0 + exp(-x));
+  return exp(x - top) / total;
+}
+
+template <typename T, int kPer>
+using Vec = T __attribute__((ext_vector_type(kPer)));
+
+// kPer neighbouring logits of a row; `whole`: rows of kLanes * kPer experts
+// that start at multiples of kPer.
+template <typename T, int kPer>
+__device__ __forceinline__ void load_logits(float (&x)[kPer], T const* row,
+                                            int at, int experts, bool whole) {
+  if (whole) {
+    if constexpr (kPer == 1) {
+      x[0] = static_cast<float>(row[at]);
+    } else {
+      auto const v = *reinterpret_cast<Vec<T, kPer> const*>(row + at);
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmax(v, __shfl_xor(v, off));
-  return v;
+      for (int i = 0; i < kPer; ++i) x[i] = static_cast<float>(v[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      x[i] = at + i < experts ? static_cast<float>(row[at + i]) : -INFINITY;
+  }
 }
 
 }  // namespace
 
-template <typename T, int kPer, bool kSigmoid>
+// kRanked: ranks are scores plus bias, or groups are chosen by scores.
+template <typename T, int kLanes, int kPer, bool kSigmoid, bool kRanked>
 __global__ __launch_bounds__(kRouteWaves * 64) void k_route(
     RouteArgs a, int64_t* __restrict__ idx_out, float* __restrict__ w_out) {
-  // keys of this wave's row, for the lanes that rank groups
-  __shared__ double ranked[kRouteWaves][kPer * 64];
+  constexpr int kTokens = 64 / kLanes;  // of a wave
+  constexpr double kInf = INFINITY;
+  __shared__ double ranked[kRanked ? kRouteWaves : 1]
+                          [kRanked ? kTokens : 1][kRanked ? kLanes * kPer : 1];
   int const wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int const t = blockIdx.x * kRouteWaves + wave;
-  if (t >= a.tokens) return;  // waves of a block share nothing
-  T const* row = static_cast<T const*>(a.logits) + t * a.stride;
+  int const sub = lane % kLanes, mine = lane / kLanes;
+  int const token = (blockIdx.x * kRouteWaves + wave) * kTokens + mine;
+  if (token - mine >= a.tokens) return;  // waves of a block share nothing
+  // lanes behind the last token go along with it
+  int const t = token < a.tokens ? token : a.tokens - 1;
+  T const* const row = static_cast<T const*>(a.logits) + t * a.stride;
+  int const e0 = sub * kPer;
 
-  double x[kPer];
-  double top = -INFINITY;
+  float x[kPer];
+  load_logits<T, kPer>(x, row, e0, a.experts, a.whole);
+  float bias[kRanked ? kPer : 1];
+  if constexpr (kRanked) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      bias[i] = a.bias ? a.bias[min(e0 + i, a.experts - 1)] : 0.f;
+  }
+  double top = 0.0, total = 1.0;
   bool nan = false;
 #pragma unroll
-  for (int v = 0; v < kPer; ++v) {
-    int const e = v * 64 + lane;
-    x[v] = e < a.experts ? load_logit(row + e) : -INFINITY;
-    nan |= x[v] != x[v];
-    top = fmax(top, x[v]);
-  }
-  bool const spoiled_nan = __ballot(nan) != 0;
-
-  bool const grouped = a.groups > 1;
-  bool const by_score = a.bias != nullptr || grouped;
-  double total = 1.0;
-  bool spoiled = spoiled_nan;
-  if (!kSigmoid) {
-    top = wave_fmax(top);
-    spoiled |= top == INFINITY;
-    if (by_score || !a.renormalize) {
+  for (int i = 0; i < kPer; ++i) nan |= x[i] != x[i];
+  uint64_t const row_lanes =
+      (kLanes == 64 ? ~0ull : (1ull << (kLanes & 63)) - 1) << mine * kLanes;
+  bool spoiled = (__ballot(nan) & row_lanes) != 0;
+  if constexpr (!kSigmoid) {
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) most = fmaxf(most, x[i]);
+    top = row_max<kLanes>(static_cast<double>(most));
+    spoiled |= top == kInf;
+    if (kRanked || !a.renormalize) {
       double sum = 0.0;
 #pragma unroll
-      for (int v = 0; v < kPer; ++v)
-        if (x[v] > -INFINITY) sum += exp(x[v] - top);
-      total = wave_sum(sum);
+      for (int i = 0; i < kPer; ++i)
+        sum += x[i] > -INFINITY ? exp(x[i] - top) : 0.0;
+      total = row_sum<kLanes>(sum);
     }
   }
 
+  // ranks: of 64 bits, or the logit and the index in one word
   uint64_t key[kPer];
-  uint64_t open_groups = ~0ull;
-  int const group_size = a.experts / a.groups;
-  if (by_score) {
+  double s[kRanked ? kPer : 1];
+  if constexpr (kRanked) {
+    bool const grouped = a.groups > 1;
 #pragma unroll
-    for (int v = 0; v < kPer; ++v) {
-      int const e = v * 64 + lane;
-      bool const open = x[v] > -INFINITY;
-      double s = 0.0;
-      if (open)
-        s = kSigmoid ? 1.0 / (1.0 + exp(-x[v])) : exp(x[v] - top) / total;
-      if (a.bias != nullptr && open) s += static_cast<double>(a.bias[e]);
-      s = open ? s : -INFINITY;
-      key[v] = key_image(a.bias != nullptr ? s : x[v]);
-      if (grouped) ranked[wave][e] = s;
+    for (int i = 0; i < kPer; ++i) {
+      int const e = e0 + i;
+      bool const open = x[i] > -INFINITY;  // also not NaN
+      // worked out for closed ones, too: without a branch the exponentials
+      // of a lane's experts overlap
+      double const score = score_of<kSigmoid>(x[i], top, total);
+      s[i] = open ? score : 0.0;
+      double const rank = open ? s[i] + bias[i] : -kInf;
+      key[i] = image(a.bias != nullptr ? rank : static_cast<double>(x[i]));
+      if (grouped) ranked[wave][mine][e] = rank == rank ? rank : -kInf;
+    }
+    if (grouped) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      // 2^n lanes for a group; each takes the best two of its share
+      int const size = a.experts / a.groups;
+      int const log_each = 31 - __builtin_clz(kLanes / a.groups);
+      int const each = 1 << log_each, g_mine = sub >> log_each;
+      double first = -kInf, second = -kInf;
+      auto add = [&](double f1, double f2) {
+        second = fmax(fmin(first, f1), fmax(second, f2));
+        first = fmax(first, f1);
+      };
+      if (g_mine < a.groups)
+        for (int i = sub & (each - 1); i < size; i += each)
+          add(ranked[wave][mine][g_mine * size + i], -kInf);
+      for (int by = 1; by < each; by <<= 1) {
+        double const f1 = __shfl_xor(first, by), f2 = __shfl_xor(second, by);
+        add(f1, f2);
+      }
+      double value = first;
+      if (a.group_best == 2 && second > -kInf) value += second;
+      int before = 0;  // groups ahead of this lane's
+      for (int g = 0; g < a.groups; ++g) {
+        double const o = __shfl(value, (g << log_each) + mine * kLanes);
+        before += o > value || (o == value && g < g_mine);
+      }
+      uint64_t const open_groups =
+          __ballot(g_mine < a.groups && before < a.topk_groups) >>
+          mine * kLanes;
+      float const by_size = 1.f / static_cast<float>(size);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        // exact: e + 1/2 is far from the next multiple for its rounding
+        int const g =
+            min(static_cast<int>((static_cast<float>(e0 + i) + 0.5f) * by_size),
+                a.groups - 1);
+        if (!((open_groups >> (g << log_each)) & 1)) key[i] = 0;
+      }
     }
   } else {
 #pragma unroll
-    for (int v = 0; v < kPer; ++v) key[v] = key_image(x[v]);
-  }
-  if (grouped) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    double first = -INFINITY, second = -INFINITY;
-    if (lane < a.groups)
-      for (int i = 0; i < group_size; ++i) {
-        double const k = ranked[wave][lane * group_size + i];
-        if (k > first) {
-          second = first;
-          first = k;
-        } else if (k > second) {
-          second = k;
-        }
-      }
-    double value = first;
-    if (a.group_best == 2 && second > -INFINITY) value += second;
-    int rank = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      double const o = __shfl(value, g);
-      rank += o > value || (o == value && g < lane);
-    }
-    open_groups = __ballot(lane < a.groups && rank < a.topk_groups);
-#pragma unroll
-    for (int v = 0; v < kPer; ++v) {
-      int const e = v * 64 + lane;
-      if (e < a.experts && !((open_groups >> (e / group_size)) & 1))
-        key[v] = 0;
+    for (int i = 0; i < kPer; ++i) {
+      uint32_t const hi = image(x[i]);
+      key[i] = hi ? static_cast<uint64_t>(hi) << 32 |
+                        ~static_cast<uint32_t>(e0 + i)
+                  : 0;
     }
   }
 
-  int picked = -1;  // lane k: the k-th pick
+  int picked = -1;  // lane `sub` of a token's: pick number `sub`
+  double s_picked = 0.0;
   for (int k = 0; k < a.topk; ++k) {
     uint64_t best = key[0];
     int at = 0;
 #pragma unroll
-    for (int v = 1; v < kPer; ++v)
-      if (key[v] > best) {
-        best = key[v];
-        at = v;
+    for (int i = 1; i < kPer; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
       }
     uint32_t const hi = static_cast<uint32_t>(best >> 32);
-    uint32_t const top_hi = wave_max(hi);
-    if (top_hi == 0) break;  // every open key's image has its high word set
-    uint64_t who = __ballot(hi == top_hi);
-    int e = at * 64 + lane;
-    if (__popcll(who) > 1) {
-      uint32_t const lo = static_cast<uint32_t>(best);
-      uint32_t const top_lo = wave_max(hi == top_hi ? lo : 0);
-      bool const tied = hi == top_hi && lo == top_lo;
-      uint32_t const first =
-          ~wave_max(tied ? ~static_cast<uint32_t>(e) : 0);
-      who = __ballot(tied && static_cast<uint32_t>(e) == first);
+    uint32_t const lo = static_cast<uint32_t>(best);
+    uint32_t const top_hi = row_max<kLanes>(hi);
+    if (__ballot(top_hi != 0) == 0) break;
+    bool cand = hi == top_hi;
+    int chosen = e0 + at;
+    uint64_t who = __ballot(cand);
+    if constexpr (kRanked) {
+      if (__popcll(who) > kTokens) {
+        uint32_t const top_lo = row_max<kLanes>(cand ? lo : 0);
+        cand &= lo == top_lo;
+        uint32_t const first = row_max<kLanes>(
+            cand ? ~static_cast<uint32_t>(chosen) : 0);
+        cand &= ~static_cast<uint32_t>(chosen) == first;
+        who = __ballot(cand);
+      }
+    } else {
+      if (__popcll(who) > kTokens) {
+        cand &= lo == row_max<kLanes>(cand ? lo : 0);
+        who = __ballot(cand);
+      }
     }
-    int const winner = __builtin_ctzll(who);
-    int const chosen = __builtin_amdgcn_readlane(e, winner);
-    if (lane == k) picked = chosen;
+    // every row with an open expert has one candidate left
+    int const winner =
+        __builtin_ctzll((who & row_lanes) | 0x8000000000000000ull);
+    if constexpr (kLanes == 64) {
+      chosen = __builtin_amdgcn_readlane(
+          chosen, __builtin_amdgcn_readfirstlane(winner));
+      if constexpr (kRanked) {
+        double sk = s[0];
 #pragma unroll
-    for (int v = 0; v < kPer; ++v)
-      if (v * 64 + lane == chosen) key[v] = 0;
+        for (int i = 1; i < kPer; ++i) sk = at == i ? s[i] : sk;
+        uint2 const w = __builtin_bit_cast(uint2, sk);
+        int const from = __builtin_amdgcn_readfirstlane(winner);
+        sk = __builtin_bit_cast(
+            double,
+            make_uint2(__builtin_amdgcn_readlane(static_cast<int>(w.x), from),
+                       __builtin_amdgcn_readlane(static_cast<int>(w.y), from)));
+        if (sub == k) s_picked = sk;
+      }
+    } else {
+      chosen = __shfl(chosen, winner);
+    }
+    bool const open = top_hi != 0;
+    if (sub == k && open) {
+      picked = chosen;
+      if constexpr (!kRanked) s_picked = from_image(top_hi);  // the logit
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (open && e0 + i == chosen) key[i] = 0;
   }
 
-  double s = 0.0;
-  if (picked >= 0) {
-    double const xk = load_logit(row + picked);
-    s = kSigmoid ? 1.0 / (1.0 + exp(-xk)) : exp(xk - top) / total;
+  // weights: lanes below topk
+  if constexpr (!kRanked || kLanes != 64) {
+    if (picked >= 0) {
+      double const xk =
+          kRanked ? static_cast<double>(static_cast<float>(row[picked]))
+                  : s_picked;
+      s_picked = score_of<kSigmoid>(xk, top, total);
+    }
   }
+  if (picked < 0) s_picked = 0.0;
   if (a.renormalize) {
-    double const sum = wave_sum(s);
-    s = sum > 0.0 ? s / sum : 0.0;
+    double const sum = row_sum<kLanes>(s_picked);
+    s_picked = sum > 0.0 ? s_picked / sum : 0.0;
   }
-  if (lane < a.topk) {
-    int64_t const o = static_cast<int64_t>(t) * a.topk + lane;
+  if (sub < a.topk && token < a.tokens) {
+    int64_t const o = static_cast<int64_t>(t) * a.topk + sub;
     idx_out[o] = picked;
-    w_out[o] = spoiled ? NAN : static_cast<float>(s * a.scale);
+    w_out[o] = spoiled ? NAN : static_cast<float>(s_picked * a.scale);
   }
 }
 
@@ -222,137 +350,186 @@ __global__ __launch_bounds__(kRouteWaves * 64) void k_route(
 //   sigmoid:                scale g_k s_k (1 - s_k)
 // Lane k works out what pick k adds; then each lane gathers, for its experts,
 // what the picks add: no atomics, and an index that occurs twice adds twice.
-template <typename T, int kPer, bool kSigmoid>
+template <typename T, int kLanes, int kPer, bool kSigmoid>
 __global__ __launch_bounds__(kRouteWaves * 64) void k_route_grad(
     RouteArgs a, float const* __restrict__ gw,
     int64_t const* __restrict__ idx, T* __restrict__ grad) {
+  constexpr int kTokens = 64 / kLanes;
+  constexpr double kInf = INFINITY;
   int const wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int const t = blockIdx.x * kRouteWaves + wave;
-  if (t >= a.tokens) return;
-  T const* row = static_cast<T const*>(a.logits) + t * a.stride;
+  int const sub = lane % kLanes, mine = lane / kLanes;
+  int const token = (blockIdx.x * kRouteWaves + wave) * kTokens + mine;
+  if (token - mine >= a.tokens) return;
+  int const t = token < a.tokens ? token : a.tokens - 1;
+  T const* const row = static_cast<T const*>(a.logits) + t * a.stride;
+  int const e0 = sub * kPer;
 
   int e_k = -1;
-  double g = 0.0, x_k = -INFINITY;
-  if (lane < a.topk) {
-    int64_t const o = static_cast<int64_t>(t) * a.topk + lane;
+  double g = 0.0, x_k = -kInf;
+  if (sub < a.topk) {
+    int64_t const o = static_cast<int64_t>(t) * a.topk + sub;
     int64_t const e = idx[o];
     if (e >= 0 && e < a.experts) {
       e_k = static_cast<int>(e);
       g = gw[o];
-      x_k = load_logit(row + e_k);
+      x_k = static_cast<float>(row[e_k]);
     }
   }
   bool const dense = !kSigmoid && !a.renormalize;
-  double x[kPer];
+  float x[kPer];
   double top = x_k, total = 1.0;
   if (dense) {
-    top = -INFINITY;
+    load_logits<T, kPer>(x, row, e0, a.experts, a.whole);
+    top = -kInf;
 #pragma unroll
-    for (int v = 0; v < kPer; ++v) {
-      int const e = v * 64 + lane;
-      x[v] = e < a.experts ? load_logit(row + e) : -INFINITY;
-      top = fmax(top, x[v]);
-    }
+    for (int i = 0; i < kPer; ++i) top = fmax(top, x[i]);
   }
-  if (!kSigmoid) top = wave_fmax(top);
+  if (!kSigmoid) top = row_max<kLanes>(top);
   if (dense) {
     total = 0.0;
 #pragma unroll
-    for (int v = 0; v < kPer; ++v)
-      if (x[v] != -INFINITY) total += exp(x[v] - top);
-    total = wave_sum(total);
+    for (int i = 0; i < kPer; ++i)
+      total += x[i] != -INFINITY ? exp(x[i] - top) : 0.0;
+    total = row_sum<kLanes>(total);
   }
   double s = 0.0;
-  if (e_k >= 0 && x_k != -INFINITY)
-    s = kSigmoid ? 1.0 / (1.0 + exp(-x_k)) : exp(x_k - top) / total;
+  if (e_k >= 0 && x_k != -kInf) s = score_of<kSigmoid>(x_k, top, total);
 
   double add, inner = 0.0;
   if (a.renormalize) {
-    double const sum = wave_sum(s);
+    double const sum = row_sum<kLanes>(s);
     double const r = sum != 0.0 ? s / sum : 0.0;
-    inner = wave_sum(g * r);
+    inner = row_sum<kLanes>(g * r);
     add = a.scale * r * (g - inner);
     if (kSigmoid) add *= 1.0 - s;
   } else if (kSigmoid) {
     add = a.scale * g * s * (1.0 - s);
   } else {
-    inner = wave_sum(g * s);
+    inner = row_sum<kLanes>(g * s);
     add = a.scale * g * s;
   }
 
   double acc[kPer];
 #pragma unroll
-  for (int v = 0; v < kPer; ++v)
-    acc[v] = dense && x[v] != -INFINITY
-                 ? -a.scale * inner * (exp(x[v] - top) / total)
+  for (int i = 0; i < kPer; ++i)
+    acc[i] = dense && x[i] != -INFINITY
+                 ? -a.scale * inner * (exp(x[i] - top) / total)
                  : 0.0;
   for (int k = 0; k < a.topk; ++k) {
-    int const e = __builtin_amdgcn_readlane(e_k, k);
-    double const more = __shfl(add, k);
-    if (e < 0) continue;
+    int const e = __shfl(e_k, mine * kLanes + k);
+    double const more = __shfl(add, mine * kLanes + k);
 #pragma unroll
-    for (int v = 0; v < kPer; ++v)
-      if (v * 64 + lane == e) acc[v] += more;
+    for (int i = 0; i < kPer; ++i) acc[i] += e == e0 + i ? more : 0.0;
   }
-  T* out = grad + static_cast<int64_t>(t) * a.experts;
+  if (token >= a.tokens) return;
+  T* const out = grad + static_cast<int64_t>(t) * a.experts + e0;
+  if (a.whole_out) {
+    if constexpr (kPer == 1) {
+      out[0] = static_cast<T>(static_cast<float>(acc[0]));
+    } else {
+      Vec<T, kPer> v;
 #pragma unroll
-  for (int v = 0; v < kPer; ++v) {
-    int const e = v * 64 + lane;
-    if (e < a.experts) out[e] = static_cast<T>(static_cast<float>(acc[v]));
+      for (int i = 0; i < kPer; ++i)
+        v[i] = static_cast<T>(static_cast<float>(acc[i]));
+      *reinterpret_cast<Vec<T, kPer>*>(out) = v;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (e0 + i < a.experts)
+        out[i] = static_cast<T>(static_cast<float>(acc[i]));
   }
 }
 
 namespace {
 
-template <typename F>
-void by_size(int experts, F&& f) {
-  if (experts <= 64) f(std::integral_constant<int, 1>{});
-  else if (experts <= 128) f(std::integral_constant<int, 2>{});
-  else if (experts <= 256) f(std::integral_constant<int, 4>{});
-  else if (experts <= 512) f(std::integral_constant<int, 8>{});
-  else f(std::integral_constant<int, 16>{});
+// 16 lanes for a token where the row and the picks fit and where 64 would
+// need more than 4 waves on each of the card's 1024 vector units.
+// (4096 and 16384 tokens measured at both ends of that bound, see below.)
+constexpr int kWideTokens = 4096;
+
+template <typename T, int kLanes, int kPer>
+void set_whole(RouteArgs& a, void const* grad) {
+  constexpr int kBytes = kPer * static_cast<int>(sizeof(T));
+  bool const full = a.experts == kLanes * kPer;
+  a.whole = full && reinterpret_cast<uintptr_t>(a.logits) % kBytes == 0 &&
+            a.stride % kPer == 0;
+  a.whole_out = full && reinterpret_cast<uintptr_t>(grad) % kBytes == 0;
+}
+
+template <typename T, typename F>
+void by_size(RouteArgs const& a, F&& f) {
+  auto const call = [&](auto lanes, auto per) { f(T{}, lanes, per); };
+#define UCCL_ROUTE(lanes, per)                       \
+  call(std::integral_constant<int, lanes>{},         \
+       std::integral_constant<int, per>{})
+  int const e = a.experts;
+  if (a.tokens > kWideTokens && e <= 256 && a.topk <= 16 && a.groups <= 16) {
+    if (e <= 16) UCCL_ROUTE(16, 1);
+    else if (e <= 32) UCCL_ROUTE(16, 2);
+    else if (e <= 64) UCCL_ROUTE(16, 4);
+    else if (e <= 128) UCCL_ROUTE(16, 8);
+    else UCCL_ROUTE(16, 16);
+  } else {
+    if (e <= 64) UCCL_ROUTE(64, 1);
+    else if (e <= 128) UCCL_ROUTE(64, 2);
+    else if (e <= 256) UCCL_ROUTE(64, 4);
+    else if (e <= 512) UCCL_ROUTE(64, 8);
+    else UCCL_ROUTE(64, 16);
+  }
+#undef UCCL_ROUTE
 }
 
 template <typename F>
-void by_elem(Elem e, F&& f) {
-  if (e == Elem::kF32) f(float{});
-  else if (e == Elem::kBF16) f(__hip_bfloat16{});
-  else f(__half{});
+void by_kind(RouteArgs const& a, F&& f) {
+  if (a.elem == Elem::kF32) by_size<float>(a, f);
+  else if (a.elem == Elem::kBF16) by_size<__bf16>(a, f);
+  else by_size<_Float16>(a, f);
+}
+
+template <int kLanes>
+int grid_of(RouteArgs const& a) {
+  constexpr int kTokens = kRouteWaves * (64 / kLanes);
+  return (a.tokens + kTokens - 1) / kTokens;
 }
 
 }  // namespace
 
-void launch_route(RouteArgs const& a, int64_t* idx, float* weights,
+void launch_route(RouteArgs const& args, int64_t* idx, float* weights,
                   hipStream_t s) {
-  int const grid = (a.tokens + kRouteWaves - 1) / kRouteWaves;
-  by_elem(a.elem, [&](auto t) {
+  by_kind(args, [&](auto t, auto lanes, auto per) {
     using T = decltype(t);
-    by_size(a.experts, [&](auto per) {
-      constexpr int kPer = decltype(per)::value;
-      if (a.sigmoid)
-        k_route<T, kPer, true>
-            <<<grid, kRouteWaves * 64, 0, s>>>(a, idx, weights);
-      else
-        k_route<T, kPer, false>
-            <<<grid, kRouteWaves * 64, 0, s>>>(a, idx, weights);
-    });
+    constexpr int kLanes = decltype(lanes)::value, kPer = decltype(per)::value;
+    RouteArgs a = args;
+    set_whole<T, kLanes, kPer>(a, nullptr);
+    int const grid = grid_of<kLanes>(a);
+    bool const ranked = a.bias != nullptr || a.groups > 1;
+    auto const go = [&](auto sigmoid, auto with_ranks) {
+      k_route<T, kLanes, kPer, decltype(sigmoid)::value,
+              decltype(with_ranks)::value>
+          <<<grid, kRouteWaves * 64, 0, s>>>(a, idx, weights);
+    };
+    if (a.sigmoid && ranked) go(std::true_type{}, std::true_type{});
+    else if (a.sigmoid) go(std::true_type{}, std::false_type{});
+    else if (ranked) go(std::false_type{}, std::true_type{});
+    else go(std::false_type{}, std::false_type{});
   });
 }
 
-void launch_route_grad(RouteArgs const& a, float const* grad_weights,
+void launch_route_grad(RouteArgs const& args, float const* grad_weights,
                        int64_t const* idx, void* grad, hipStream_t s) {
-  int const grid = (a.tokens + kRouteWaves - 1) / kRouteWaves;
-  by_elem(a.elem, [&](auto t) {
+  by_kind(args, [&](auto t, auto lanes, auto per) {
     using T = decltype(t);
-    by_size(a.experts, [&](auto per) {
-      constexpr int kPer = decltype(per)::value;
-      if (a.sigmoid)
-        k_route_grad<T, kPer, true><<<grid, kRouteWaves * 64, 0, s>>>(
-            a, grad_weights, idx, static_cast<T*>(grad));
-      else
-        k_route_grad<T, kPer, false><<<grid, kRouteWaves * 64, 0, s>>>(
-            a, grad_weights, idx, static_cast<T*>(grad));
-    });
+    constexpr int kLanes = decltype(lanes)::value, kPer = decltype(per)::value;
+    RouteArgs a = args;
+    set_whole<T, kLanes, kPer>(a, grad);
+    int const grid = grid_of<kLanes>(a);
+    if (a.sigmoid)
+      k_route_grad<T, kLanes, kPer, true><<<grid, kRouteWaves * 64, 0, s>>>(
+          a, grad_weights, idx, static_cast<T*>(grad));
+    else
+      k_route_grad<T, kLanes, kPer, false><<<grid, kRouteWaves * 64, 0, s>>>(
+          a, grad_weights, idx, static_cast<T*>(grad));
   });
 }
 

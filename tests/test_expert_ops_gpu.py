@@ -398,6 +398,35 @@ def test_matmul_16bit(e, r, length, n, k, expected, kind, turned, dtype, out):
     check_product(got, x0, w.double(), mask)
 
 
+@pytest.mark.parametrize("expected", [1, 16, 17, 40, 64, 65, 128, 200])
+@pytest.mark.parametrize("dtype", [F8, BF, HF])
+def test_matmul_expected_rows(dtype, expected):
+    """The hint changes how the product is computed, never what."""
+    e, r, length, n, k = 40, 3, 23, 1032, 384
+    g = gen(expected)
+    counts = some_counts(g, e, r, length, "random")
+    mask = mask_of(counts, r * length)
+    y = torch.full((e, r * length, n), 7.0, dtype=BF, device="cuda")
+    before = y.clone()
+    if dtype == F8:
+        x, xs = rows_to_8bit(randn(g, e, r * length, k))
+        w, ws = weights_to_8bit(randn(g, e, n, k) * 0.05)
+        x.view(torch.uint8)[~mask] = 0x7F
+        xs[~mask] = math.nan
+        ep.expert_matmul(x, w, counts, x_scales=xs, w_scales=ws, out=y,
+                         expected_rows=expected)
+        x0, w0 = values_of(x, xs, 1), values_of(w, ws, 128)
+    else:
+        k = 376
+        x = randn(g, e, r * length, k).to(dtype)
+        w = (randn(g, e, n, k) * 0.05).to(dtype)
+        x[~mask] = math.nan
+        ep.expert_matmul(x, w, counts, out=y, expected_rows=expected)
+        x0, w0 = x.double(), w.double()
+    x0 = torch.where(mask[..., None], x0, 0.0)
+    check_product(y, x0, w0, mask, dtype == F8, before)
+
+
 def test_matmul_odd_n_16bit():
     g = gen(5)
     for n in (1, 3, 17, 255, 259):

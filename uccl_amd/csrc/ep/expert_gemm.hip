@@ -803,6 +803,208 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   }
 }
 
+// Few rows: bound by the weights, which are read once, straight into the
+// registers of the wave that multiplies them. A block has 16 TP columns of an
+// expert; its waves share the contraction, a quarter each, so that all of a
+// small product's weights are on their way at once, and join their sums
+// through LDS in a fixed order. The rows, 64 at a time, come from the caches.
+constexpr int kRowWaves = 4;
+
+template <Elem kElem, int TP, int NQ>
+struct RowPart {
+  i32x8 p[TP], q[NQ];
+  float s[NQ];
+  float sw;
+};
+
+template <Elem kElem, Elem kOut, int TP, int NQ>
+__device__ __forceinline__ void multiply_rows(
+    GemmArgs const& a, char const* const (&p_at)[TP],
+    char const* const (&q_at)[4], char const* const (&qs_at)[4],
+    float const* ps_at, int begin, int end, f32x4* joined, int wave, int lane) {
+  constexpr bool k8 = kElem == Elem::kF8;
+  constexpr int kSize = k8 ? 1 : 2;
+  // steps on their way: what 256 registers hold
+  constexpr int kDeep = NQ == 1 ? 4 : NQ == 2 ? 3 : 2;
+  int const bytes = a.depth * kSize;
+  int const low = (lane >> 4) * 16, high = low + 64;  // of a step
+  char const* const zeros = reinterpret_cast<char const*>(&zero_page);
+  auto load16 = [&](char const* row, int at) {
+    char const* const g = k8 || at < bytes ? row + at : zeros;
+    return *reinterpret_cast<i32x4 const*>(g);
+  };
+  auto load = [&](RowPart<kElem, TP, NQ>& r, int step) {
+    auto operand = [&](char const* row) {
+      return __builtin_shufflevector(load16(row, step * kStep + low),
+                                     load16(row, step * kStep + high), 0, 1, 2,
+                                     3, 4, 5, 6, 7);
+    };
+#pragma unroll
+    for (int i = 0; i < TP; ++i) r.p[i] = operand(p_at[i]);
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      r.q[j] = operand(q_at[j]);
+      if constexpr (k8)
+        r.s[j] = *reinterpret_cast<float const*>(qs_at[j] + step * 4);
+    }
+    if constexpr (k8) r.sw = ps_at[step];
+  };
+  f32x4 acc[TP][NQ];
+#pragma unroll
+  for (int i = 0; i < TP; ++i)
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto add = [&](RowPart<kElem, TP, NQ> const& r) {
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      float const s = k8 ? r.s[j] * r.sw : 1.f;
+#pragma unroll
+      for (int i = 0; i < TP; ++i) {
+        if constexpr (k8) {
+          f32x4 const d = mfma8(r.p[i], r.q[j]);
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            acc[i][j][v] = fmaf(d[v], s, acc[i][j][v]);
+        } else {
+          acc[i][j] =
+              mfma16<kElem>(half<0>(r.p[i]), half<0>(r.q[j]), acc[i][j]);
+          acc[i][j] =
+              mfma16<kElem>(half<1>(r.p[i]), half<1>(r.q[j]), acc[i][j]);
+        }
+      }
+    }
+  };
+  RowPart<kElem, TP, NQ> part[kDeep];
+#pragma unroll
+  for (int n = 0; n < kDeep; ++n)
+    if (begin + n < end) load(part[n], begin + n);
+  for (int step = begin; step < end; step += kDeep) {
+#pragma unroll
+    for (int n = 0; n < kDeep; ++n) {
+      if (step + n < end) add(part[n]);
+      if (step + n + kDeep < end) load(part[n], step + n + kDeep);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TP; ++i)
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+      joined[((i * NQ + j) * kRowWaves + wave) * 64 + lane] = acc[i][j];
+}
+
+template <Elem kElem, Elem kOut, int TP>
+__global__ __launch_bounds__(kRowWaves * 64, 2) void k_expert_rows(
+    GemmArgs a) {
+  constexpr bool k8 = kElem == Elem::kF8;
+  constexpr int kSize = k8 ? 1 : 2;
+  constexpr int kOutSize = kOut == Elem::kF32 ? 4 : 2;
+  __shared__ f32x4 joined[TP * 4 * kRowWaves * 64];
+  __shared__ int ends[kMaxSlotCells];
+  int const wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int const e = blockIdx.y, p0 = blockIdx.x * (16 * TP);
+  int const sources = a.rows.sources;
+
+  // valid rows up to and with each source
+  int valid = a.rows.length;
+  if (a.rows.counts) {
+    if (wave == 0) {
+      int carry = 0;
+      for (int s0 = 0; s0 < sources; s0 += 64) {
+        int v = s0 + lane < sources
+                    ? min(max(a.rows.counts[e * sources + s0 + lane], 0),
+                          a.rows.length)
+                    : 0;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          int const o = __shfl_up(v, off);
+          if (lane >= off) v += o;
+        }
+        if (s0 + lane < sources) ends[s0 + lane] = carry + v;
+        carry += __shfl(v, 63);
+      }
+    }
+    __syncthreads();
+    valid = ends[sources - 1];
+  }
+  auto slot = [&](int i) {
+    if (!a.rows.counts) return i;
+    int begin = 0;
+    for (int s = 0; s < sources; ++s) {
+      int const end = ends[s];
+      if (i < end) return s * a.rows.length + i - begin;
+      begin = end;
+    }
+    return 0;
+  };
+
+  char const* const pe = a.p + e * a.p_expert;
+  char const* const qe = a.q + e * a.q_expert;
+  char const* p_at[TP];
+#pragma unroll
+  for (int i = 0; i < TP; ++i)
+    p_at[i] = pe + static_cast<int64_t>(
+                       min(p0 + i * 16 + (lane & 15), a.np - 1)) *
+                       a.p_row;
+  float const* ps_at = nullptr;
+  if constexpr (k8)
+    ps_at = reinterpret_cast<float const*>(a.p_scales + e * a.ps_expert +
+                                           p0 / 128 * a.ps_row);
+  int const steps = (a.depth * kSize + kStep - 1) / kStep;
+  int const begin = steps * wave / kRowWaves;
+  int const end = steps * (wave + 1) / kRowWaves;
+
+  for (int q0 = 0; q0 < valid; q0 += 64) {
+    int const tiles = min(4, (valid - q0 + 15) / 16);
+    char const* q_at[4];
+    char const* qs_at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < tiles) {
+        int64_t const row = slot(min(q0 + j * 16 + (lane & 15), valid - 1));
+        q_at[j] = qe + row * a.q_row;
+        if constexpr (k8)
+          qs_at[j] = a.q_scales + e * a.qs_expert + row * a.qs_row;
+      }
+    auto go = [&](auto n) {
+      multiply_rows<kElem, kOut, TP, decltype(n)::value>(
+          a, p_at, q_at, qs_at, ps_at, begin, end, joined, wave, lane);
+    };
+    if (tiles == 1) go(std::integral_constant<int, 1>{});
+    else if (tiles == 2) go(std::integral_constant<int, 2>{});
+    else if (tiles == 3) go(std::integral_constant<int, 3>{});
+    else go(std::integral_constant<int, 4>{});
+    __syncthreads();
+    for (int t = wave; t < TP * tiles; t += kRowWaves) {
+      int const i = t / tiles, j = t - i * tiles;
+      f32x4 sum = joined[t * kRowWaves * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < kRowWaves; ++w)
+        sum += joined[(t * kRowWaves + w) * 64 + lane];
+      int const q = q0 + j * 16 + (lane & 15);
+      int const p = p0 + i * 16 + (lane >> 4) * 4;
+      if (q < valid && p < a.np) {
+        char* const o = a.out + e * a.out_expert + slot(q) * a.out_row +
+                        static_cast<int64_t>(p) * kOutSize;
+        using T = OutType<kOut>;
+        if (a.wide && p + 4 <= a.np) {
+          struct alignas(4 * kOutSize) Four {
+            T v[4];
+          } four;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) four.v[v] = static_cast<T>(sum[v]);
+          *reinterpret_cast<Four*>(o) = four;
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (p + v < a.np)
+              reinterpret_cast<T*>(o)[v] = static_cast<T>(sum[v]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
 int compute_units() {
   int dev = 0, n = 0;
   UCCL_CHECK_HIP(hipGetDevice(&dev));
@@ -829,11 +1031,42 @@ void launch_tiles(GemmArgs const& a, int blocks_per_cu, hipStream_t s) {
       <<<static_cast<int>(grid), WP * WQ * 64, 0, s>>>(a);
 }
 
+template <Elem kElem, Elem kOut, int TP>
+void launch_rows(GemmArgs const& a, hipStream_t s) {
+  dim3 const grid((a.np + 16 * TP - 1) / (16 * TP), a.rows.experts);
+  k_expert_rows<kElem, kOut, TP><<<grid, kRowWaves * 64, 0, s>>>(a);
+}
+
+// Which kernel: by the rows that an expert is expected to have, and whether
+// tiles of 128 columns give every compute unit one. Measured in us, 8 bits:
+//   32 experts, 4096 x 7168      rows of an expert:   8    16    32    64
+//     k_expert_rows                                 171   212   284
+//     tiles of 256 x 64                                         170   212
+//     tiles of 256 x 256                            252   255   253   256
+//   1 expert, 7168 x 2048        rows:                1    16    64
+//     k_expert_rows                                 5.5   7.6  16.4
+//     tiles of 128 x 128                           20.0  20.1  20.4
 template <Mode kMode, Elem kElem, Elem kOut>
 void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
-  int64_t const tiles = static_cast<int64_t>(a.rows.experts) *
-                        ((a.np + 255) / 256) * ((expected_rows + 255) / 256);
-  if (tiles >= compute_units())
+  auto tiles = [&](int p, int q) {
+    return static_cast<int64_t>(a.rows.experts) * ((a.np + p - 1) / p) *
+           ((expected_rows + q - 1) / q);
+  };
+  int const cus = compute_units();
+  if constexpr (kMode == Mode::kProduct) {
+    if (expected_rows <= 16 || (expected_rows <= 64 && tiles(128, 64) < cus)) {
+      if (tiles(32, 64) >= 4 * cus)
+        launch_rows<kElem, kOut, 2>(a, s);
+      else
+        launch_rows<kElem, kOut, 1>(a, s);
+      return;
+    }
+  }
+  if constexpr (kMode != Mode::kWeightGrad) {
+    if (expected_rows <= 64)
+      return launch_tiles<kMode, kElem, kOut, 256, 64, 4, 1>(a, 1, s);
+  }
+  if (tiles(256, 256) >= cus)
     launch_tiles<kMode, kElem, kOut, 256, 256, 4, 2>(a, 1, s);
   else
     launch_tiles<kMode, kElem, kOut, 128, 128, 2, 2>(a, 2, s);

@@ -427,6 +427,87 @@ def test_matmul_expected_rows(dtype, expected):
     check_product(y, x0, w0, mask, dtype == F8, before)
 
 
+@pytest.mark.parametrize("kind, out", [("product", BF), ("product", F32),
+                                       ("turned", BF), ("turned", F32),
+                                       ("8 bit", BF), ("8 bit", HF)])
+def test_matmul_more_tiles_than_compute_units(kind, out):
+    """Several tiles for each block, the last of them half empty."""
+    e, r, length, n, k = 20, 3, 210, 1304, 328
+    g = gen(len(kind))
+    counts = some_counts(g, e, r, length, "random")
+    counts[3:9] = length
+    mask = mask_of(counts, r * length)
+    y = torch.full((e, r * length, n), 7.0, dtype=out, device="cuda")
+    before = y.clone()
+    if kind == "8 bit":
+        k = 384
+        x, xs = rows_to_8bit(randn(g, e, r * length, k))
+        w, ws = weights_to_8bit(randn(g, e, n, k) * 0.05)
+        ep.expert_matmul(x, w, counts, x_scales=xs, w_scales=ws, out=y)
+        x0, w0 = values_of(x, xs, 1), values_of(w, ws, 128)
+    else:
+        x = randn(g, e, r * length, k).to(BF)
+        w = (randn(g, e, n, k) * 0.05).to(BF)
+        if kind == "turned":
+            w = w.transpose(1, 2).contiguous().transpose(1, 2)
+        x[~mask] = math.nan
+        ep.expert_matmul(x, w, counts, out=y)
+        x0, w0 = x.double(), w.double()
+    x0 = torch.where(mask[..., None], x0, 0.0)
+    check_product(y, x0, w0, mask, kind == "8 bit", before)
+
+
+@pytest.mark.parametrize("kind", ["product", "turned", "8 bit", "wgrad"])
+def test_rows_of_an_expert_span_more_than_4_gib(kind):
+    slots, n, k = 4200, 520, 264
+    pitch = 1 << 19
+    g = gen(len(kind))
+    counts = torch.tensor([slots - 3], dtype=torch.int32, device="cuda")
+    mask = mask_of(counts[None], slots)[0]
+
+    def far(rows):  # [1, slots, cols], the rows `pitch` elements apart
+        wide = torch.empty(slots, pitch * (2 if rows.dtype == F8 else 1),
+                           dtype=rows.dtype, device="cuda")
+        wide[:, :rows.shape[1]] = rows
+        return wide[None, :, :rows.shape[1]]
+
+    if kind == "8 bit":
+        k = 256
+        x, xs = rows_to_8bit(randn(g, 1, slots, k))
+        w, ws = weights_to_8bit(randn(g, 1, n, k) * 0.05)
+        got = ep.expert_matmul(far(x[0]), w, counts, x_scales=xs, w_scales=ws)
+        check_product(got, values_of(x, xs, 1), values_of(w, ws, 128),
+                      mask[None], True)
+        return
+    x = randn(g, slots, k).to(BF)
+    if kind == "wgrad":
+        grad = (randn(g, slots, n) * 0.05).to(BF)
+        got = ep.expert_weight_grad(far(grad), far(x), counts)
+        gt = grad.double()[mask].t().contiguous()[None]
+        check_product(got, gt, x.double()[mask].t().contiguous()[None],
+                      torch.ones(1, n, dtype=torch.bool, device="cuda"))
+        return
+    w = (randn(g, 1, n, k) * 0.05).to(BF)
+    if kind == "turned":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    got = ep.expert_matmul(far(x), w, counts)
+    check_product(got, x.double()[None], w.double(), mask[None])
+
+
+def test_matmul_weights_far_apart():
+    """Rows of weights so far apart that a tile's span more than 4 GiB."""
+    n, k, pitch = 300, 72, 1 << 23
+    g = gen(3)
+    wide = torch.empty(n, pitch, dtype=BF, device="cuda")
+    wide[:, :k] = randn(g, n, k) * 0.05
+    w = wide[None, :, :k]
+    x = randn(g, 1, 200, k).to(BF)
+    every = torch.ones(1, 200, dtype=torch.bool, device="cuda")
+    for rows in (1, 200):
+        check_product(ep.expert_matmul(x, w, expected_rows=rows), x.double(),
+                      w.double(), every)
+
+
 def test_matmul_odd_n_16bit():
     g = gen(5)
     for n in (1, 3, 17, 255, 259):

@@ -54,32 +54,45 @@ constexpr int kStep = 128;  // bytes of the contraction in a stage, a row
 __device__ const int4 zero_page = {0, 0, 0, 0};
 
 // --- loads to LDS ----------------------------------------------------------
-// Each lane loads 16 (4) bytes from its own address to LDS at `lds` + kAt +
-// lane * 16 (* 4), where `on` is not 0. `on` and `lds` are uniform. The
-// instruction has no register result; the wave waits for it in a barrier
-// below before the LDS is read. The branch is inside the statement so that it
-// does not cut the block that the compiler schedules.
-
-template <int kAt>
-__device__ __forceinline__ void lds_load16(int on, char const* base,
-                                           uint32_t offset, uint32_t lds) {
-  asm volatile(
-      "s_cmp_eq_u32 %4, 0\n\ts_cbranch_scc1 1f\n\ts_add_u32 m0, %2, %3\n\t"
-      "s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n1:"
-      :
-      : "v"(offset), "s"(base), "s"(lds), "n"(kAt), "s"(on)
-      : "memory", "m0", "scc");
+// Each lane loads 16 bytes from its own address to LDS at `lds` + lane * 16;
+// load n of a group to n KiB behind that, and n KiB behind its offset.
+// Where `on` is 0 it loads nothing. The branch is inside the statement so that
+// it does not cut the block that the compiler schedules.
+#define LDS_LOAD_GROUP(loads, last, ...)                                      \
+  asm volatile("s_cmp_eq_u32 %1, 0\n\ts_cbranch_scc1 1f\n\t"                  \
+               "s_mov_b32 m0, %2\n\ts_nop 0\n\t" loads "\n1:"               \
+               :                                                              \
+               : "s"(base), "s"(on), "s"(lds), "n"(last), __VA_ARGS__         \
+               : "memory", "m0", "scc")
+template <int kCount>
+__device__ __forceinline__ void lds_load_group(int on, char const* base,
+                                               uint32_t const* off,
+                                               uint32_t lds) {
+  static_assert(kCount == 1 || kCount == 2 || kCount == 4, "loads of a group");
+  if constexpr (kCount == 1)
+    LDS_LOAD_GROUP("global_load_lds_dwordx4 %4, %0", 0, "v"(off[0]));
+  else if constexpr (kCount == 2)
+    LDS_LOAD_GROUP(
+        "global_load_lds_dwordx4 %4, %0\n\t"
+        "global_load_lds_dwordx4 %5, %0 offset:%3",
+        1024, "v"(off[0]), "v"(off[1]));
+  else
+    LDS_LOAD_GROUP(
+        "global_load_lds_dwordx4 %4, %0\n\t"
+        "global_load_lds_dwordx4 %5, %0 offset:1024\n\t"
+        "global_load_lds_dwordx4 %6, %0 offset:2048\n\t"
+        "global_load_lds_dwordx4 %7, %0 offset:%3",
+        3 * 1024, "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]));
 }
-template <int kAt>
-__device__ __forceinline__ void lds_load16(int on, char const* g,
-                                           uint32_t lds) {
+#undef LDS_LOAD_GROUP
+__device__ __forceinline__ void lds_load16(char const* g, uint32_t lds) {
   asm volatile(
-      "s_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 1f\n\ts_add_u32 m0, %1, %2\n\t"
-      "s_nop 0\n\tglobal_load_lds_dwordx4 %0, off\n1:"
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
       :
-      : "v"(g), "s"(lds), "n"(kAt), "s"(on)
-      : "memory", "m0", "scc");
+      : "v"(g), "s"(lds)
+      : "memory", "m0");
 }
+// 4 bytes a lane, where `on` is not 0.
 __device__ __forceinline__ void lds_load4(int on, char const* g,
                                           uint32_t lds) {
   asm volatile(
@@ -150,6 +163,7 @@ struct GemmArgs {
   int np;     // extent of p
   int nq;     // extent of q (weight gradient only; else the valid rows)
   int depth;  // contraction in elements (product only)
+  bool near;  // a lane's addresses in a stage lie within 32 bits
   bool wide;  // 8 results of a row can be stored together
   char const* q_scales;
   char const* p_scales;
@@ -320,7 +334,8 @@ __device__ __forceinline__ i32x4 half(i32x8 v) {
 // P rows are given to MFMA rows so that a lane's results of two tiles are 8
 // consecutive p: row m of tile i is p = 32 (i / 2) + 8 (m / 4) + 4 (i % 2) +
 // m % 4 of the wave's 64.
-template <Mode kMode, Elem kElem, Elem kOut, int BP, int BQ, int WP, int WQ>
+template <Mode kMode, Elem kElem, Elem kOut, int BP, int BQ, int WP, int WQ,
+          bool kFar>
 __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   constexpr bool kWGrad = kMode == Mode::kWeightGrad;
   constexpr bool kPTurned = kMode != Mode::kProduct;
@@ -336,7 +351,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   constexpr int kPLoads = kPBytes / 1024 / kWaves;  // of a wave and stage
   constexpr int kQLoads = kQBytes / 1024 / kWaves;
   constexpr int kHalf = kQLoads / 2;
-  constexpr int kFirst = kPLoads + kHalf, kLoads = kPLoads + kQLoads;
+  constexpr int kLoads = kPLoads + kQLoads;
   static_assert(kPLoads * 1024 * kWaves == kPBytes, "P loads");
   static_assert(kHalf * 2048 * kWaves == kQBytes, "Q loads");
   constexpr int kOutSize = kOut == Elem::kF32 ? 4 : 2;
@@ -353,7 +368,10 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   __shared__ RowTable table;
   // rows of a tile: of the last, whose results are stored, of this one and of
   // the next; weight gradient: rows of a stage, 4 stages in a ring
-  __shared__ int slots[kWGrad ? 4 : 3][kWGrad ? kDepth : BQ];
+  constexpr int kNoted = 8;
+  __shared__ int slots[kWGrad ? kNoted : 3][kWGrad ? kDepth : BQ];
+  __shared__ uint32_t p_rows[kWGrad ? kNoted : 1][kWGrad ? kDepth : 1];
+  __shared__ uint32_t q_rows[kWGrad ? kNoted : 1][kWGrad ? kDepth : 1];
 
   int const wave = uniform(threadIdx.x >> 6);
   int const lane = threadIdx.x & 63;
@@ -365,11 +383,17 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   int const total =
       uniform(kWGrad ? a.rows.experts * tiles_p * ((a.nq + BQ - 1) / BQ)
                      : table.tile_end[a.rows.experts - 1] * tiles_p);
-  // Blocks are handed to the 8 XCDs in turn. Each round of tiles is cut into
-  // one run for each XCD, so that the blocks that share an L2 share operands,
-  // and all of the card works on neighbouring tiles, whose operands stay in
-  // the last-level cache.
-  int tile = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  // Blocks are handed to the 8 XCDs in turn. Each round of tiles, the last one
+  // too, is cut into one run for each XCD, so that the blocks that share an L2
+  // share operands, all XCDs have work, and all of the card works on
+  // neighbouring tiles, whose operands stay in the last-level cache.
+  auto tile_of = [&](int first) {  // of the round that begins there, or total
+    int const round = min(total - first, static_cast<int>(gridDim.x));
+    int const run = (round + 7) >> 3, i = blockIdx.x >> 3;
+    int const t = (blockIdx.x & 7) * run + i;
+    return i < run && t < round ? first + t : total;
+  };
+  int first = 0, tile = tile_of(0);
   if (tile >= total) return;
 
   // --- this lane's part of the loads ---------------------------------------
@@ -393,53 +417,59 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
       return (at % (kQPitch / 16)) ^ (((row & 3) << 2) & (kQPitch / 16 - 1));
     return (at & 7) ^ ((row >> 1) & 7);
   };
+  char const* const zeros = reinterpret_cast<char const*>(&zero_page);
   // row (or column) of the tile that place r of half h belongs to
   auto q_of = [&](int h, int r) {
     return r / (RQ / 2) * RQ + h * (RQ / 2) + r % (RQ / 2);
   };
 
-  char const* const zeros = reinterpret_cast<char const*>(&zero_page);
+  // Of the tile that is loaded. Loads of whole stages take 32-bit offsets from
+  // a base that moves along the contraction. Up to four loads share an LDS
+  // address: load n of a group lands n KiB behind it, and reads n KiB behind
+  // its offset, which is that much lower; kBias keeps it above 0.
+  constexpr uint32_t kBias = 4096;
+  constexpr int kGroup = kPLoads / 2;
+  Tile from{};
+  int from_turn = 0;
   char const* p_base = nullptr;
-  uint32_t p_off[kPLoads];
-  char const* p_at[kPLoads];
-  char const* q_at[kQLoads];
+  char const* q_base = nullptr;
+  uint32_t p_off[kPLoads], q_off[kQLoads];
   char const* scale_at = nullptr;
-  int steps = 0, depth = 0;
+  int steps = 0, whole = 0, depth = 0;
 
-  // addresses of a tile's first stage
+  // offsets of a tile's first stage
   auto set_tile = [&](Tile const& t, int turn) {
-    char const* const pe = a.p + t.e * a.p_expert;
-    char const* const qe = a.q + t.e * a.q_expert;
+    from = t;
+    from_turn = turn;
     depth = kWGrad ? t.valid : a.depth;
     steps = uniform((depth + kDepth - 1) / kDepth);
-    // Rows of weights lie within 32 bits of the tile's first; gathered rows
-    // need not.
-    p_base = pe + static_cast<int64_t>(t.p0) * a.p_row;
+    whole = uniform(a.near ? depth / kDepth : 0);
+    p_base = a.p + t.e * a.p_expert - kBias;
+    p_base += kPTurned ? static_cast<int64_t>(t.p0) * 2
+                       : static_cast<int64_t>(t.p0) * a.p_row;
+    q_base = a.q + t.e * a.q_expert - kBias;
+    if constexpr (kQTurned) q_base += static_cast<int64_t>(t.q0) * 2;
+    uint32_t const p_pitch = static_cast<uint32_t>(a.p_row);
+    uint32_t const q_pitch = static_cast<uint32_t>(a.q_row);
 #pragma unroll
     for (int j = 0; j < kPLoads; ++j) {
-      if constexpr (k8)
-        p_off[j] = static_cast<uint32_t>(min(p_row(j), a.np - 1 - t.p0)) *
-                       static_cast<uint32_t>(a.p_row) +
-                   p_chunk(j) * 16;
-      else if constexpr (!kPTurned)
-        p_at[j] = pe +
-                  static_cast<int64_t>(min(t.p0 + p_row(j), a.np - 1)) *
-                      a.p_row +
-                  p_chunk(j) * 16;
+      uint32_t const at = kBias - j % kGroup * 1024;
+      if constexpr (!kPTurned)
+        p_off[j] = min(p_row(j), a.np - 1 - t.p0) * p_pitch + p_chunk(j) * 16 +
+                   at;
       else  // columns behind the last give results that are not stored
-        p_at[j] = pe + static_cast<int64_t>(kWGrad ? 0 : p_row(j)) * a.p_row +
-                  min(t.p0 + p_chunk(j) * 8, a.np - 8) * 2;
+        p_off[j] = (kWGrad ? 0 : p_row(j) * p_pitch) +
+                   min(p_chunk(j) * 8, a.np - 8 - t.p0) * 2 + at;
     }
 #pragma unroll
     for (int j = 0; j < kQLoads; ++j) {
-      if constexpr (!kQTurned) {
-        int const row = q_of(j / kHalf, q_row(j));
-        q_at[j] = qe + static_cast<int64_t>(slots[turn][row]) * a.q_row +
-                  q_chunk(j) * 16;
-      } else {
-        int const col = t.q0 + q_of(j / kHalf, q_chunk(j) * 8);
-        q_at[j] = qe + min(col, a.nq - 8) * 2;
-      }
+      uint32_t const at = kBias - j % kHalf * 1024;
+      if constexpr (!kQTurned)
+        q_off[j] = slots[turn][q_of(j / kHalf, q_row(j))] * q_pitch +
+                   q_chunk(j) * 16 + at;
+      else
+        q_off[j] = min(q_of(j / kHalf, q_chunk(j) * 8), a.nq - 8 - t.q0) * 2 +
+                   at;
     }
     if constexpr (k8) {
       if (wave < BQ / 64) {
@@ -447,7 +477,8 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
                    static_cast<int64_t>(slots[turn][threadIdx.x % BQ]) *
                        a.qs_row;
       } else {
-        int const block = min(t.p0 + min(lane, BP / 128 - 1) * 128, a.np - 1) / 128;
+        int const block =
+            min(t.p0 + min(lane, BP / 128 - 1) * 128, a.np - 1) / 128;
         scale_at = a.p_scales + t.e * a.ps_expert + block * a.ps_row;
       }
     }
@@ -455,47 +486,83 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
 
   uint32_t const my_p = lds0 + wave * kPLoads * 1024;
   uint32_t const my_q = lds0 + kPBytes + wave * kHalf * 1024;
-  // Load n of stage `step`: P, then the two halves of Q.
-  auto load_part = [&](auto n, int on, int step)
+  // Weight gradient: where a stage's rows begin.
+  uint32_t p_at[kWGrad ? kPLoads : 1], q_at[kWGrad ? kQLoads : 1];
+  auto find_rows = [&](int step) __attribute__((always_inline)) {
+    if constexpr (kWGrad) {
+#pragma unroll
+      for (int j = 0; j < kPLoads; ++j)
+        p_at[j] = p_off[j] + p_rows[step % kNoted][p_row(j)];
+#pragma unroll
+      for (int j = 0; j < kQLoads; ++j)
+        q_at[j] = q_off[j] + q_rows[step % kNoted][q_row(j)];
+    }
+  };
+  // Loads of stage `step`: parts 0 and 1 are P, 2 and 3 the halves of Q.
+  // A wave's first loads of a stage are counted on to be done in this order.
+  auto load_near = [&](auto n, int on, int step)
                        __attribute__((always_inline)) {
-    constexpr int j = decltype(n)::value;
+    constexpr int part = decltype(n)::value;
     uint32_t const buf = (step & 1) * kStage;
-    if constexpr (j < kPLoads) {
-      if constexpr (k8) {
-        lds_load16<j * 1024>(on, p_base, p_off[j], my_p + buf);
-        if (j == kPLoads - 1) p_base += kStep;
-      } else {
-        char const* g;
-        if constexpr (!kPTurned) {
-          g = step * kStep + p_chunk(j) * 16 < depth * kSize ? p_at[j] : zeros;
-          p_at[j] += kStep;
-        } else {
-          int const row = p_row(j);
-          if constexpr (kWGrad) {
-            g = p_at[j] +
-                static_cast<int64_t>(slots[step & 3][row]) * a.p_row;
-          } else {
-            g = p_at[j];
-            p_at[j] += kDepth * a.p_row;
-          }
-          g = step * kDepth + row < depth ? g : zeros;
-        }
-        lds_load16<j * 1024>(on, g, my_p + buf);
-      }
+    if constexpr (part < 2) {
+      uint32_t const* const off = kWGrad ? p_at : p_off;
+      lds_load_group<kGroup>(on, p_base, off + part * kGroup,
+                             my_p + buf + part * kGroup * 1024);
+      if constexpr (part == 1 && !kPTurned) p_base += kStep;
+      if constexpr (part == 1 && kPTurned && !kWGrad)
+        p_base += kDepth * a.p_row;
     } else {
-      constexpr int k = j - kPLoads;
-      char const* g;
-      if constexpr (!kQTurned) {
-        g = k8 || step * kStep + q_chunk(k) * 16 < depth * kSize ? q_at[k]
-                                                                : zeros;
-        q_at[k] += kStep;
-      } else {
-        int const row = q_row(k);
-        g = q_at[k] + static_cast<int64_t>(slots[step & 3][row]) * a.q_row;
-        g = step * kDepth + row < depth ? g : zeros;
+      uint32_t const* const off = kWGrad ? q_at : q_off;
+      lds_load_group<kHalf>(on, q_base, off + (part - 2) * kHalf,
+                            my_q + buf + (part - 2) * (kQBytes / 2));
+      if constexpr (part == 3 && !kQTurned) q_base += kStep;
+    }
+  };
+  auto load_part = [&](auto n, int step) __attribute__((always_inline)) {
+    constexpr int part = decltype(n)::value;
+    static_assert(part >= 0 && part < 4);
+    uint32_t const buf = (step & 1) * kStage;
+    if constexpr (k8 && !kFar) {  // all stages are whole
+      load_near(n, before(step, steps), step);
+    } else if (!kFar && step < whole) {
+      load_near(n, -1, step);
+    } else if (step < steps) {
+      // A stage that the contraction ends in, or rows too far apart: full
+      // addresses, zeros behind the end. The rows of a weight gradient often
+      // have few stages, so its loads go out together.
+      auto row_at = [&](char const* base, int64_t row, int64_t pitch) {
+        return base + row * pitch;
+      };
+      char const* const pe = a.p + from.e * a.p_expert;
+      char const* const qe = a.q + from.e * a.q_expert;
+      int64_t const along = static_cast<int64_t>(step) * kStep;
+#pragma unroll(kWGrad ? 4 : 1)
+      for (int n = 0; n < (part < 2 ? kGroup : kHalf); ++n) {
+        int const j = part < 2 ? part * kGroup + n : n;
+        int const row = part < 2 ? p_row(j) : q_row(j);
+        int const chunk = part < 2 ? p_chunk(j) : q_chunk(j);
+        bool const turned_in = step * kDepth + row < depth;
+        bool const direct_in = step * kStep + chunk * 16 < depth * kSize;
+        char const* g;
+        if constexpr (part < 2 && !kPTurned)
+          g = row_at(pe, min(from.p0 + row, a.np - 1), a.p_row) + along +
+              chunk * 16;
+        else if constexpr (part < 2)
+          g = row_at(pe,
+                     kWGrad ? slots[step % kNoted][row] : step * kDepth + row,
+                     a.p_row) +
+              min(from.p0 + chunk * 8, a.np - 8) * 2;
+        else if constexpr (!kQTurned)
+          g = row_at(qe, slots[from_turn][q_of(part - 2, row)], a.q_row) +
+              along + chunk * 16;
+        else
+          g = row_at(qe, slots[step % kNoted][row], a.q_row) +
+              min(from.q0 + q_of(part - 2, chunk * 8), a.nq - 8) * 2;
+        bool const in =
+            (part < 2 ? kPTurned : kQTurned) ? turned_in : direct_in;
+        uint32_t const to = part < 2 ? my_p : my_q + (part - 2) * (kQBytes / 2);
+        lds_load16(in ? g : zeros, uniform(to + buf + j * 1024));
       }
-      lds_load16<(k / kHalf) * (kQBytes / 2) + (k % kHalf) * 1024>(
-          on, g, my_q + buf);
     }
   };
   // A step's scales, 4 steps in a ring: the first BQ / 64 waves load those of
@@ -528,8 +595,12 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
             seg_begin = seg_end;
             seg_end = table.end[t.e * a.rows.sources + seg];
           }
-          slots[step & 3][threadIdx.x] =
-              seg * a.rows.length + i - seg_begin;
+          uint32_t const slot = seg * a.rows.length + i - seg_begin;
+          slots[step % kNoted][threadIdx.x] = slot;
+          p_rows[step % kNoted][threadIdx.x] =
+              slot * static_cast<uint32_t>(a.p_row);
+          q_rows[step % kNoted][threadIdx.x] =
+              slot * static_cast<uint32_t>(a.q_row);
         }
       }
     }
@@ -543,8 +614,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   // The first two stages of a tile whose rows are noted.
   auto begin_tile = [&](Tile const& t, int turn) {
     if constexpr (kWGrad) {
-      note_slots(t, 0);
-      note_slots(t, 1);
+      for (int step = 0; step < 3; ++step) note_slots(t, step);
     }
     // slots are noted, and nobody reads the stages any more
     stage_barrier<kLoads, kLoads + kStores>(0);
@@ -552,9 +622,10 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
       int const on = before(step, steps);
-      unrolled<0, kFirst>([&](auto n) { load_part(n, on, step); });
+      find_rows(step);
+      unrolled<0, 3>([&](auto n) { load_part(n, step); });
       load_scales(on, step);
-      unrolled<kFirst, kLoads>([&](auto n) { load_part(n, on, step); });
+      load_part(std::integral_constant<int, 3>{}, step);
     }
   };
 
@@ -648,7 +719,8 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
     // The next tile is looked up while the first stage is on its way.
     Tile const done = now;
     int const next_turn = turn < 2 ? turn + 1 : 0;
-    tile += gridDim.x;
+    first += gridDim.x;
+    tile = tile_of(first);
     bool const more = tile < total;
     if (more) {
       now = find_tile<kMode, BP, BQ>(a, table, tile, tiles_p);
@@ -670,8 +742,8 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
         sw = lds_read<float>(lds_addr(p_scale) + (step & 3) * 256 +
                              wp * RP / 128 * 4);
       int const on = before(step + 2, steps);
-      if constexpr (kWGrad)
-        if (on) note_slots(done, step + 2);
+      note_slots(done, step + 3);
+      find_rows(step + 2);
       // Twice in a step, when all waves have read what lies in P and the
       // first half of Q, and in the second, the loads of the stage after
       // next take their places; so loads have a step and a half to land.
@@ -718,21 +790,13 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
             read_p(step + 1, i * 2 - 3);
           }
         }
-        if constexpr (t >= kMid && t < kEnd) {
-          constexpr int u = (t - kMid) * 2, kU = kEnd - kMid;  // early
-          unrolled<less(u * kFirst / kU, kFirst),
-                   less((u + 2) * kFirst / kU, kFirst)>(
-              [&](auto n) __attribute__((always_inline)) {
-                load_part(n, on, step + 2);
-              });
-          if constexpr (t == kEnd - 1) load_scales(on, step + 2);
-        } else if constexpr (t >= kEnd) {
-          constexpr int u = t - kEnd;
-          unrolled<kFirst + u * kHalf / TP, kFirst + (u + 1) * kHalf / TP>(
-              [&](auto n) __attribute__((always_inline)) {
-                load_part(n, on, step + 2);
-              });
-        }
+        // part 0 from kMid on, part 3 behind the barrier of kEnd
+        constexpr int kGap = (kEnd - kMid) / 3;
+        if constexpr (t == kMid || t == kMid + kGap || t == kMid + 2 * kGap)
+          load_part(std::integral_constant<int, (t - kMid) / kGap>{}, step + 2);
+        if constexpr (t == kEnd)
+          load_part(std::integral_constant<int, 3>{}, step + 2);
+        if constexpr (t == kEnd - 1) load_scales(on, step + 2);
         __builtin_amdgcn_sched_barrier(0);
       });
     }
@@ -749,9 +813,9 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
 
     // The next tile's first loads go out before this one's results.
     if (more) begin_tile(now, next_turn);
+    int const out_p = done.p0 + wp * RP + (lane >> 4) * 8;
     char* const out = a.out + done.e * a.out_expert +
-                      static_cast<int64_t>(done.p0 + wp * RP + (lane >> 4) * 8) *
-                          kOutSize;
+                      static_cast<int64_t>(out_p) * kOutSize;
     auto row_of = [&](int j) {
       if constexpr (!kQTurned)
         return wq * RQ + j * 16 + (lane & 15);
@@ -789,7 +853,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
         char* const o = out + row * a.out_row;
 #pragma unroll
         for (int i = 0; i < TP; i += 2) {
-          int const n = a.np - (done.p0 + wp * RP + (lane >> 4) * 8 + i * 16);
+          int const n = a.np - (out_p + i * 16);
           if (n >= 8 && a.wide)
             store8<kOut>(o + i * 16 * kOutSize, acc[i][j], acc[i + 1][j]);
           else
@@ -1013,12 +1077,20 @@ int compute_units() {
   return n;
 }
 
+// Whether the offsets of a stage's loads from the tile's first address, with
+// the loads' own share of them, fit 32 bits: `p_span` and `q_span` rows.
+bool lies_near(GemmArgs const& a, int64_t p_span, int64_t q_span) {
+  constexpr int64_t kEnd = (int64_t{1} << 32) - 16384;
+  return p_span * a.p_row < kEnd && q_span * a.q_row < kEnd;
+}
+
 bool stores_wide(GemmArgs const& a) {
   return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row % 16 == 0 &&
          a.out_expert % 16 == 0;
 }
 
-template <Mode kMode, Elem kElem, Elem kOut, int BP, int BQ, int WP, int WQ>
+template <Mode kMode, Elem kElem, Elem kOut, int BP, int BQ, int WP, int WQ,
+          bool kFar = false>
 void launch_tiles(GemmArgs const& a, int blocks_per_cu, hipStream_t s) {
   int64_t const tiles_p = (a.np + BP - 1) / BP;
   int64_t const q = kMode == Mode::kWeightGrad
@@ -1027,7 +1099,7 @@ void launch_tiles(GemmArgs const& a, int blocks_per_cu, hipStream_t s) {
   int64_t const most = a.rows.experts * tiles_p * ((q + BQ - 1) / BQ);
   int64_t grid = std::min<int64_t>(most, compute_units() * blocks_per_cu);
   grid = (grid + 7) / 8 * 8;
-  k_expert_gemm<kMode, kElem, kOut, BP, BQ, WP, WQ>
+  k_expert_gemm<kMode, kElem, kOut, BP, BQ, WP, WQ, kFar>
       <<<static_cast<int>(grid), WP * WQ * 64, 0, s>>>(a);
 }
 
@@ -1037,15 +1109,23 @@ void launch_rows(GemmArgs const& a, hipStream_t s) {
   k_expert_rows<kElem, kOut, TP><<<grid, kRowWaves * 64, 0, s>>>(a);
 }
 
-// Which kernel: by the rows that an expert is expected to have, and whether
-// tiles of 128 columns give every compute unit one. Measured in us, 8 bits:
-//   32 experts, 4096 x 7168      rows of an expert:   8    16    32    64
-//     k_expert_rows                                 171   212   284
-//     tiles of 256 x 64                                         170   212
-//     tiles of 256 x 256                            252   255   253   256
-//   1 expert, 7168 x 2048        rows:                1    16    64
-//     k_expert_rows                                 5.5   7.6  16.4
-//     tiles of 128 x 128                           20.0  20.1  20.4
+// Which kernel, by the rows that an expert is expected to have and the tiles
+// that this makes. Measured in us:
+//   32 experts, 4096 x 7168, 8 bits      rows:   8    16    32    64   128
+//     k_expert_rows                            171   212   284
+//     tiles of 256 x 64                                    172   215   309
+//     tiles of 256 x 128                                   190   197   256
+//     tiles of 256 x 256                       252   255   253   266   271
+//   1 expert, 7168 x 2048, 8 bits        rows:   1    16    64
+//     k_expert_rows                            5.5   7.6  16.4
+//     tiles of 128 x 128                      20.0  20.1  20.4
+//   8 experts, 256 rows    1024 x 1024, 16 bits   2048 x 1024, 8 bits
+//     tiles of 128 x 128                  15.2                   26.4
+//     tiles of 256 x 128                  19.9                   16.4
+//   weight gradient, 8 experts, 139 rows  1000 x 1024, 16 bits
+//     tiles of 128 x 128                  17.2
+//     tiles of 256 x 128                  12.5
+//     tiles of 256 x 256                  15.8
 template <Mode kMode, Elem kElem, Elem kOut>
 void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
   auto tiles = [&](int p, int q) {
@@ -1062,14 +1142,22 @@ void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
       return;
     }
   }
+  if constexpr (kElem == Elem::kF8) {
+    if (!a.near)
+      return launch_tiles<kMode, kElem, kOut, 128, 128, 2, 2, true>(a, 2, s);
+  }
   if constexpr (kMode != Mode::kWeightGrad) {
-    if (expected_rows <= 64)
+    if (tiles(128, 128) <= cus / 2)
+      return launch_tiles<kMode, kElem, kOut, 128, 128, 2, 2>(a, 2, s);
+    if (expected_rows <= 48)
       return launch_tiles<kMode, kElem, kOut, 256, 64, 4, 1>(a, 1, s);
+    if (expected_rows <= 96)
+      return launch_tiles<kMode, kElem, kOut, 256, 128, 4, 2>(a, 1, s);
   }
   if (tiles(256, 256) >= cus)
     launch_tiles<kMode, kElem, kOut, 256, 256, 4, 2>(a, 1, s);
   else
-    launch_tiles<kMode, kElem, kOut, 128, 128, 2, 2>(a, 2, s);
+    launch_tiles<kMode, kElem, kOut, 256, 128, 4, 2>(a, 1, s);
 }
 
 template <Mode kMode, Elem kElem>
@@ -1099,6 +1187,8 @@ void launch_expert_matmul(MatmulArgs const& m, hipStream_t s) {
   a.out_expert = m.out.expert_stride * out_size;
   a.out_row = m.out.row_stride * out_size;
   a.np = m.n;
+  int64_t const slots = static_cast<int64_t>(m.rows.sources) * m.rows.length;
+  a.near = lies_near(a, 256, slots);
   a.wide = stores_wide(a);
   a.depth = m.k;
   if (m.elem == Elem::kF8) {
@@ -1138,6 +1228,8 @@ void launch_expert_weight_grad(WeightGradArgs const& w, hipStream_t s) {
   a.out_expert = w.out.expert_stride * out_size;
   a.out_row = w.out.row_stride * out_size;
   a.np = w.k;
+  int64_t const slots = static_cast<int64_t>(w.rows.sources) * w.rows.length;
+  a.near = lies_near(a, slots, slots);
   a.wide = stores_wide(a);
   a.nq = w.n;
   if (w.elem == Elem::kBF16)

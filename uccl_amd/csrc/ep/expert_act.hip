@@ -195,6 +195,32 @@ __device__ __forceinline__ double group_max(double v) {
   return v;
 }
 
+// Whether one of the values is below -85: among negative values, the order of
+// the bits. A negative NaN counts too.
+template <typename T>
+__device__ __forceinline__ bool ends_exp(x8<T> v) {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x8 const bits = __builtin_bit_cast(u16x8, v);
+  u16x4 const four = __builtin_elementwise_max(
+      __builtin_shufflevector(bits, bits, 0, 1, 2, 3),
+      __builtin_shufflevector(bits, bits, 4, 5, 6, 7));
+  u16x2 const two = __builtin_elementwise_max(
+      __builtin_shufflevector(four, four, 0, 1),
+      __builtin_shufflevector(four, four, 2, 3));
+  constexpr unsigned short kEnd =
+      __builtin_bit_cast(unsigned short, static_cast<T>(-85.f));
+  return two[0] > kEnd || two[1] > kEnd;
+}
+
+// Four values as 8-bit ones, each times `by`.
+__device__ __forceinline__ unsigned to_8bit(float a, float b, float c, float d,
+                                            float by) {
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a * by, b * by, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c * by, d * by, v, true);
+}
+
 // The j-th of 16 values, of two lots of 8.
 template <typename T>
 __device__ __forceinline__ float pick(x8<T> const (&v)[2], int j) {
@@ -275,7 +301,7 @@ __global__ __launch_bounds__(256) void k_swiglu_quant(SwigluArgs a) {
 #pragma unroll
     for (int k = 0; k < kShares; ++k) {
       f32x8 const x = floats<T>(raw.x[k]), b = floats<T>(raw.b[k]);
-      float most = -1.f, second = -1.f, lowest = 0.f;
+      float most = -1.f, second = -1.f;
       top_x[k] = top_b[k] = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -287,9 +313,8 @@ __global__ __launch_bounds__(256) void k_swiglu_quant(SwigluArgs a) {
         top_b[k] = more ? b[j] : top_b[k];
         second = __builtin_amdgcn_fmed3f(second, size, most);
         most = fmaxf(most, size);
-        lowest = fminf(lowest, x[j]);
       }
-      float const group = group_max(lowest < -85.f ? INFINITY : most);
+      float const group = group_max(ends_exp<T>(raw.x[k]) ? INFINITY : most);
       wild[k] = !(group >= 1e-20f && group <= 1e30f);
       limit[k] = group * (1.f - 0x1p-15f);
       if (s[k].on) {
@@ -314,18 +339,13 @@ __global__ __launch_bounds__(256) void k_swiglu_quant(SwigluArgs a) {
       exact[0] = fmax(exact[0], j < 8 ? size : 0.0);
       exact[1] = fmax(exact[1], j < 8 ? 0.0 : size);
     }
-    // 20 bits of a float lie behind the 3 of an 8-bit value. Where they are
-    // within kNear of one half, 32 bits do not decide: the error above, and
-    // 2 units of the scaling, are at most 96 of those bits.
-    constexpr unsigned kNear = 112;
+    // Scaled values are known to 96 parts in 2^24: the error above, and that
+    // of the scaling. Where a value less 2^-17 of it and the value and 2^-17
+    // of it become the same 8-bit value, it is that one; else 32 bits do not
+    // decide.
+    constexpr float kNear = 0x1p-17f;
+    unsigned values[kShares][2];
     float scale[kShares];
-    auto behind = [](float y) {
-      float const size = fabsf(y);
-      // below 2^-6 the steps no longer shrink
-      float const fixed = size < 0x1p-6f ? size + 0x1p-6f : size;
-      return (__builtin_bit_cast(unsigned, fixed) + 0x80000u + kNear) &
-             0xfffffu;
-    };
     unsigned near = 0;
 #pragma unroll
     for (int k = 0; k < kShares; ++k) {
@@ -338,16 +358,20 @@ __global__ __launch_bounds__(256) void k_swiglu_quant(SwigluArgs a) {
               ? static_cast<float>(largest < INFINITY ? q : largest)
               : 1.f;
       float const inverse = __builtin_amdgcn_rcpf(scale[k]);
-      unsigned nearest = ~0u;
+      unsigned differ[2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[k][j] *= inverse;
-        nearest = min(nearest, behind(v[k][j]));
+      for (int d = 0; d < 2; ++d) {
+        auto const scaled = [&](float by) {
+          return to_8bit(v[k][d * 4], v[k][d * 4 + 1], v[k][d * 4 + 2],
+                         v[k][d * 4 + 3], by);
+        };
+        values[k][d] = scaled(inverse * (1.f - kNear));
+        differ[d] = values[k][d] ^ scaled(inverse * (1.f + kNear));
       }
-      if (s[k].on && (nearest <= 2 * kNear || wild[k])) {
+      if (s[k].on && ((differ[0] | differ[1]) != 0 || wild[k])) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (behind(v[k][j]) <= 2 * kNear || wild[k])
+          if ((differ[j / 4] >> (j % 4 * 8) & 0xffu) || wild[k])
             near |= 1u << (k * 8 + j);
       }
     }
@@ -357,22 +381,20 @@ __global__ __launch_bounds__(256) void k_swiglu_quant(SwigluArgs a) {
       float const y =
           nearest_exact(silu_mul_exact(pick<T>(raw.x, j), pick<T>(raw.b, j)) /
                         (j < 8 ? scale[0] : scale[1]));
+      unsigned const place = 0xffu << (j & 3) * 8;
+      unsigned const value = to_8bit(y, y, y, y, 1.f) & place;
 #pragma unroll
       for (int k = 0; k < kShares; ++k)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[k][i] = j == k * 8 + i ? y : v[k][i];
+        for (int d = 0; d < 2; ++d)
+          if ((j >> 2) == k * 2 + d)
+            values[k][d] = (values[k][d] & ~place) | value;
     }
 #pragma unroll
     for (int k = 0; k < kShares; ++k) {
       if (!s[k].on) continue;
-      int lo = 0, hi = 0;
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][0], v[k][1], lo, false);
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][2], v[k][3], lo, true);
-      hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][4], v[k][5], hi, false);
-      hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][6], v[k][7], hi, true);
       char* const out = row_at(out_cell, a.out, s[k].at, 1);
-      *reinterpret_cast<int2*>(out + s[k].col) = make_int2(lo, hi);
+      *reinterpret_cast<uint2*>(out + s[k].col) = make_uint2(values[k][0], values[k][1]);
       if ((threadIdx.x & 15) == 0)
         reinterpret_cast<float*>(
             row_at(scale_cell, a.scales, s[k].at, 4))[s[k].col / 128] =

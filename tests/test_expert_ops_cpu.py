@@ -219,3 +219,34 @@ def test_no_gradient_is_lost():
     refused("h requires grad", ep.expert_swiglu, x)
     with torch.no_grad():
         refused("must be on GPU", ep.expert_matmul, x, w)
+
+
+def test_results_that_require_grad_are_refused():
+    x, w = torch.zeros(2, 6, 32, dtype=BF), torch.zeros(2, 24, 32, dtype=BF)
+
+    def leaf(*shape):
+        return torch.zeros(*shape, dtype=BF, requires_grad=True)
+
+    refused("out requires grad", ep.expert_matmul, x, w, out=leaf(2, 6, 24))
+    refused("out requires grad", ep.expert_weight_grad, x, x,
+            out=leaf(2, 32, 32))
+    refused("out requires grad", ep.expert_swiglu, x, out=leaf(2, 6, 16))
+    refused("out requires grad", ep.expert_swiglu_grad, x[..., :16], x,
+            out=leaf(2, 6, 32))
+
+
+def test_sizes_that_32_bits_do_not_count_are_refused():
+    def wide(*shape):  # one element, repeated
+        return torch.zeros(1, dtype=BF).expand(*shape)
+
+    long = 1 << 29
+    refused("too large", ep.expert_matmul, wide(1, 1, long), wide(1, 8, long),
+            out=torch.zeros(1, 1, 8, dtype=BF))
+    refused("too large", ep.expert_matmul, wide(1, 1, 8), wide(1, long, 8),
+            out=wide(1, 1, long))
+    refused("too large|too many slots", ep.expert_matmul, wide(1, 2 * long, 8),
+            wide(1, 8, 8), out=wide(1, 2 * long, 8))
+    refused("too large", ep.expert_weight_grad, wide(1, 1, 8),
+            wide(1, 1, long), out=wide(1, 8, long))
+    refused("too many slots", ep.expert_swiglu, wide(1, 2 * long, 16),
+            out=wide(1, 2 * long, 8))

@@ -119,7 +119,7 @@ ep::SlotRows rows_of(at::Tensor const& x, OptTensor const& counts) {
   TORCH_CHECK(experts >= 1 && experts <= ep::kMaxSlotExperts,
               "uccl_amd: 1 to ", ep::kMaxSlotExperts, " experts, got ",
               experts);
-  TORCH_CHECK(experts * slots < (int64_t(1) << 31),
+  TORCH_CHECK(experts * slots < (int64_t(1) << 30),
               "uccl_amd: too many slots");
   int64_t sources = 1;
   if (counts) {
@@ -154,8 +154,10 @@ void check_16bit(at::Tensor const& t, char const* name) {
               t.scalar_type());
 }
 
+// What the kernels count in 32 bits: rows and columns with a tile's behind
+// them, bytes of a row, tiles.
 void check_tiles(int64_t experts, int64_t a, int64_t b) {
-  TORCH_CHECK(a < (int64_t(1) << 30) && b < (int64_t(1) << 31) &&
+  TORCH_CHECK(a < (int64_t(1) << 29) && b < (int64_t(1) << 30) &&
                   experts * ((a + 15) / 16) * ((b + 15) / 16) <
                       (int64_t(1) << 31),
               "uccl_amd: the product is too large");
@@ -295,7 +297,7 @@ void expert_matmul(at::Tensor x, at::Tensor w, OptTensor counts,
   TORCH_CHECK(n >= 1 && k >= 1, "uccl_amd: w has no rows or no columns");
   check_shape(out, {experts, slots, n}, "out");
   check_tiles(experts, n, slots);
-  TORCH_CHECK(k < (int64_t(1) << 30), "uccl_amd: the product is too large");
+  TORCH_CHECK(k < (int64_t(1) << 29), "uccl_amd: the product is too large");
   TORCH_CHECK(expected_rows >= 0, "uccl_amd: expected_rows is negative");
 
   ep::MatmulArgs a{};
@@ -376,6 +378,7 @@ void expert_weight_grad(at::Tensor grad, at::Tensor x, OptTensor counts,
               "8, got ", n, " and ", k);
   check_shape(out, {experts, n, k}, "out");
   check_tiles(experts, n, k);
+  TORCH_CHECK(k < (int64_t(1) << 29), "uccl_amd: the product is too large");
   ep::WeightGradArgs a{};
   a.rows = rows_of(x, counts);
   a.grad = mat_of(grad, "grad_out");

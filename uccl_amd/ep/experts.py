@@ -99,7 +99,7 @@ def route_grad(grad_weights: torch.Tensor, logits: torch.Tensor,
     of its weights (float32) and the picks it returned. An index outside
     [0, E) adds nothing; one that occurs twice in a row adds twice. The picks
     themselves, and so the bias, have no gradient."""
-    C = _native(grad_weights=grad_weights, logits=logits)
+    C = _native(grad_weights=grad_weights, logits=logits, out=out)
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype,
                           device=logits.device)
@@ -132,10 +132,10 @@ def expert_matmul(x: torch.Tensor, w: torch.Tensor,
     as it lies (its N, the weights' K, a multiple of 8).
 
     ``expected_rows``: how many rows an expert is expected to have, by which
-    the tile is chosen (default: all its slots). It changes the speed, never
-    which rows are computed.
+    the kernel is chosen (default: all its slots). It changes the speed and
+    the order of the sums, never which rows are computed.
     """
-    C = _native(x=x, w=w)
+    C = _native(x=x, w=w, x_scales=x_scales, w_scales=w_scales, out=out)
     if out is None:
         if out_dtype is None:
             out_dtype = x.dtype if x.element_size() == 2 else torch.bfloat16
@@ -161,7 +161,7 @@ def expert_weight_grad(grad_out: torch.Tensor, x: torch.Tensor,
     has their dtype, or ``out_dtype`` (bfloat16, float16, float32). Sums are
     held in 32 bits and taken in the order of the rows. An expert without
     valid rows gets zeros."""
-    C = _native(grad_out=grad_out, x=x)
+    C = _native(grad_out=grad_out, x=x, out=out)
     if out is None:
         out = torch.empty(*x.shape[:-2], grad_out.shape[-1], x.shape[-1],
                           dtype=out_dtype or x.dtype, device=x.device)
@@ -185,7 +185,7 @@ def expert_swiglu(h: torch.Tensor, counts: Optional[torch.Tensor] = None, *,
     an 8-bit expert_matmul: scale = max |v| / 448 over each 128 columns (1 if
     all are 0), values the nearest to v / scale, ties to even, decided as if v
     were exact."""
-    C = _native(h=h)
+    C = _native(h=h, out=out, out_scales=out_scales)
     cols = h.shape[-1] // 2
     if out is None:
         out = torch.empty(*h.shape[:-1], cols, device=h.device,
@@ -208,7 +208,7 @@ def expert_swiglu_grad(grad_out: torch.Tensor, h: torch.Tensor,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of expert_swiglu's h, [E, slots, 2 * I] in its dtype, from
     grad_out [E, slots, I] of the same dtype."""
-    C = _native(grad_out=grad_out, h=h)
+    C = _native(grad_out=grad_out, h=h, out=out)
     if out is None:
         out = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     C.ep_expert_swiglu_grad(_slots(grad_out), _slots(h), _counts(counts, h),

@@ -239,14 +239,18 @@ def test_sizes_that_32_bits_do_not_count_are_refused():
     def wide(*shape):  # one element, repeated
         return torch.zeros(1, dtype=BF).expand(*shape)
 
-    long = 1 << 29
+    long = 1 << 28
     refused("too large", ep.expert_matmul, wide(1, 1, long), wide(1, 8, long),
             out=torch.zeros(1, 1, 8, dtype=BF))
     refused("too large", ep.expert_matmul, wide(1, 1, 8), wide(1, long, 8),
             out=wide(1, 1, long))
-    refused("too large|too many slots", ep.expert_matmul, wide(1, 2 * long, 8),
-            wide(1, 8, 8), out=wide(1, 2 * long, 8))
+    refused("too large|too many slots", ep.expert_matmul, wide(1, 4 * long, 8),
+            wide(1, 8, 8), out=wide(1, 4 * long, 8))
     refused("too large", ep.expert_weight_grad, wide(1, 1, 8),
             wide(1, 1, long), out=wide(1, 8, long))
-    refused("too many slots", ep.expert_swiglu, wide(1, 2 * long, 16),
-            out=wide(1, 2 * long, 8))
+    refused("too many slots", ep.expert_swiglu, wide(1, 4 * long, 16),
+            out=wide(1, 4 * long, 8))
+    row = torch.zeros(1, 8).expand(1 << 25, 8)
+    idx = torch.zeros(1, 2, dtype=torch.int64).expand(1 << 25, 2)
+    refused("too many tokens", ep.route_grad, row[:, :2], row, idx,
+            out=row)

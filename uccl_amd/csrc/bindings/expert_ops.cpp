@@ -155,9 +155,9 @@ void check_16bit(at::Tensor const& t, char const* name) {
 }
 
 // What the kernels count in 32 bits: rows and columns with a tile's behind
-// them, bytes of a row, tiles.
+// them, bytes of a row, tiles, threads for 16 columns each.
 void check_tiles(int64_t experts, int64_t a, int64_t b) {
-  TORCH_CHECK(a < (int64_t(1) << 29) && b < (int64_t(1) << 30) &&
+  TORCH_CHECK(a < (int64_t(1) << 28) && b < (int64_t(1) << 30) &&
                   experts * ((a + 15) / 16) * ((b + 15) / 16) <
                       (int64_t(1) << 31),
               "uccl_amd: the product is too large");
@@ -177,7 +177,8 @@ ep::RouteArgs route_args(at::Tensor const& logits, int64_t topk,
   TORCH_CHECK(experts >= 1 && experts <= ep::kMaxRouteExperts,
               "uccl_amd: 1 to ", ep::kMaxRouteExperts, " experts, got ",
               experts);
-  TORCH_CHECK(logits.size(0) < (int64_t(1) << 31),
+  // 64 lanes a token, and less than 2^32 lanes of a launch
+  TORCH_CHECK(logits.size(0) < (int64_t(1) << 25),
               "uccl_amd: too many tokens");
   TORCH_CHECK(topk >= 1 && topk <= std::min<int64_t>(experts,
                                                      ep::kMaxRouteTopk),
@@ -297,7 +298,7 @@ void expert_matmul(at::Tensor x, at::Tensor w, OptTensor counts,
   TORCH_CHECK(n >= 1 && k >= 1, "uccl_amd: w has no rows or no columns");
   check_shape(out, {experts, slots, n}, "out");
   check_tiles(experts, n, slots);
-  TORCH_CHECK(k < (int64_t(1) << 29), "uccl_amd: the product is too large");
+  TORCH_CHECK(k < (int64_t(1) << 28), "uccl_amd: the product is too large");
   TORCH_CHECK(expected_rows >= 0, "uccl_amd: expected_rows is negative");
 
   ep::MatmulArgs a{};
@@ -378,7 +379,7 @@ void expert_weight_grad(at::Tensor grad, at::Tensor x, OptTensor counts,
               "8, got ", n, " and ", k);
   check_shape(out, {experts, n, k}, "out");
   check_tiles(experts, n, k);
-  TORCH_CHECK(k < (int64_t(1) << 29), "uccl_amd: the product is too large");
+  TORCH_CHECK(k < (int64_t(1) << 28), "uccl_amd: the product is too large");
   ep::WeightGradArgs a{};
   a.rows = rows_of(x, counts);
   a.grad = mat_of(grad, "grad_out");

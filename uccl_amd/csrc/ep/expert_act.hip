@@ -128,10 +128,13 @@ template <typename T>
 __device__ __forceinline__ f32x8 floats(x8<T> v) {
   return __builtin_convertvector(v, f32x8);
 }
+// Past the caches, where results would take the place of what is still to be
+// read: 16384 rows of 2048 columns, 49 -> 47 us, gradient 84 -> 74 us. (Loads
+// past the caches cost 10%.)
 template <typename T>
 __device__ __forceinline__ void store8(char* row, int col, f32x8 v) {
-  reinterpret_cast<x8<T>*>(row)[col / kUnit] =
-      __builtin_convertvector(v, x8<T>);
+  __builtin_nontemporal_store(__builtin_convertvector(v, x8<T>),
+                              reinterpret_cast<x8<T>*>(row) + col / kUnit);
 }
 
 // exp(-|a| / 2), good to about a unit in the last place: the part of the

@@ -197,6 +197,9 @@ def test_route_strided_and_empty():
                         topk_groups=4)),
     (4100, 256, 17, {}),
     (4100, 300, 5, dict(renormalize=False)),
+    (32771, 256, 8, dict(scoring="sigmoid", bias=1, num_groups=8,
+                         topk_groups=4)),
+    (32770, 200, 8, dict(bias=1)),
 ])
 def test_route_many_tokens(tokens, experts, topk, kw, dtype):
     """A token's picks, weights and gradient do not hang on how many others

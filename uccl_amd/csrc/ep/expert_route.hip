@@ -444,9 +444,20 @@ __global__ __launch_bounds__(kRouteWaves * 64) void k_route_grad(
 namespace {
 
 // 16 lanes for a token where the row and the picks fit and where 64 would
-// need more than 4 waves on each of the card's 1024 vector units.
-// (4096 and 16384 tokens measured at both ends of that bound, see below.)
-constexpr int kWideTokens = 4096;
+// need more than 4 waves on each of the card's 1024 vector units; more than 32
+// where a lane would hold 16 ranks of 64 bits. Measured in us, 64 / 16 lanes:
+//   tokens                              2048         4096         8192
+//     128 experts, top 8, bf16        4.0 / 5.5    5.1 / 5.6    7.5 / 6.3
+//       gradient                      3.2 / 3.6    4.1 / 3.7    6.0 / 4.2
+//     256 experts, ranked, 8 groups   7.4 / 13.4  10.6 / 13.7  17.5 / 18.9
+//   tokens                             16384        65536
+//     128 experts, top 8, bf16       12.4 / 8.8   42.4 / 25.8
+//       gradient                      9.8 / 6.0   31.9 / 17.8
+//     256 experts, ranked, 8 groups  29.5 / 31.4   105 / 94
+// One token of the last takes 5.7: a chain of 8 picks, a few reductions each.
+// 4096 tokens read and write 4.6 MB, 0.9 us of a copy; what bounds them is
+// the 64-bit exponentials and the picks' reductions.
+constexpr int kWideTokens = 4096, kWideRanked = 32768;
 
 template <typename T, int kLanes, int kPer>
 void set_whole(RouteArgs& a, void const* grad) {
@@ -464,7 +475,9 @@ void by_size(RouteArgs const& a, F&& f) {
   call(std::integral_constant<int, lanes>{},         \
        std::integral_constant<int, per>{})
   int const e = a.experts;
-  if (a.tokens > kWideTokens && e <= 256 && a.topk <= 16 && a.groups <= 16) {
+  bool const ranked = a.bias != nullptr || a.groups > 1;
+  int const wide = ranked && e > 128 ? kWideRanked : kWideTokens;
+  if (a.tokens > wide && e <= 256 && a.topk <= 16 && a.groups <= 16) {
     if (e <= 16) UCCL_ROUTE(16, 1);
     else if (e <= 32) UCCL_ROUTE(16, 2);
     else if (e <= 64) UCCL_ROUTE(16, 4);

@@ -430,6 +430,35 @@ def test_matmul_expected_rows(dtype, expected):
     check_product(y, x0, w0, mask, dtype == F8, before)
 
 
+@pytest.mark.parametrize("k", [64, 136, 1024])
+@pytest.mark.parametrize("length, n", [(300, 1032), (65, 3), (1000, 17)])
+@pytest.mark.parametrize("kind", ["random", "full", "one", "none"])
+def test_matmul_of_middling_sizes(kind, length, n, k):
+    g = gen(k + n)
+    counts = some_counts(g, 4, 1, length, kind)
+    mask = mask_of(counts, length)
+    y = torch.full((4, length, n), 7.0, dtype=BF, device="cuda")
+    for eight in (False, True):
+        if eight and k % 128:
+            continue
+        y.fill_(7.0)
+        before = y.clone()
+        if eight:
+            x, xs = rows_to_8bit(randn(g, 4, length, k))
+            w, ws = weights_to_8bit(randn(g, 4, n, k) * 0.05)
+            x.view(torch.uint8)[~mask] = 0x7F
+            ep.expert_matmul(x, w, counts, x_scales=xs, w_scales=ws, out=y)
+            x0, w0 = values_of(x, xs, 1), values_of(w, ws, 128)
+        else:
+            x = randn(g, 4, length, k).to(BF)
+            w = (randn(g, 4, n, k) * 0.05).to(BF)
+            x[~mask] = math.nan
+            ep.expert_matmul(x, w, counts, out=y)
+            x0, w0 = x.double(), w.double()
+        x0 = torch.where(mask[..., None], x0, 0.0)
+        check_product(y, x0, w0, mask, eight, before)
+
+
 @pytest.mark.parametrize("kind, out", [("product", BF), ("product", F32),
                                        ("turned", BF), ("turned", F32),
                                        ("8 bit", BF), ("8 bit", HF)])

@@ -21,6 +21,16 @@
 // Rows behind an expert's last are never read: tiles are cut from the number
 // of valid rows, lanes behind the last row load it again, and lanes behind
 // the end of the contraction load from a page of zeros.
+//
+// What bounds a large product is LDS: a step of a 256 x 256 tile brings 64 KB
+// in and gives 192 KB to the waves, 2048 clocks of the 128 bytes it moves in
+// each, and the same 2048 clocks the matrix units are busy. 16384 rows of 8
+// experts, bf16: product 7168 x 4096 806 us, 1.19 PFLOP/s, its row gradient
+// 830 us, weight gradient 4096 x 7168 848 us, 1.13 PFLOP/s; 32768 rows, 4096 x
+// 7168, 8 bits: 917 us, 2.10 PFLOP/s. (The card's library reaches 1.40 and
+// 2.73 on dense products of 8192 cubed.) Products of few rows are bound by the
+// weights' bytes: 1024 rows of 32 experts, 4096 x 7168, 8 bits: 171 us, 5.5
+// TB/s.
 
 #include <hip/hip_runtime.h>
 

@@ -489,9 +489,12 @@ def test_matmul_more_tiles_than_compute_units(kind, out):
     check_product(y, x0, w0, mask, kind == "8 bit", before)
 
 
-@pytest.mark.parametrize("kind", ["product", "turned", "8 bit", "wgrad"])
+@pytest.mark.parametrize("kind", ["product", "turned", "8 bit", "wgrad",
+                                  "wider wgrad"])
 def test_rows_of_an_expert_span_more_than_4_gib(kind):
     slots, n, k = 4200, 520, 264
+    if kind == "wider wgrad":
+        kind, n, k = "wgrad", 2056, 1032
     pitch = 1 << 19
     g = gen(len(kind))
     counts = torch.tensor([slots - 3], dtype=torch.int32, device="cuda")
@@ -664,6 +667,55 @@ def test_weight_grad(e, r, length, n, k, kind, dtype, out):
     close(got, want, tol, "weight gradient")
     # the same again, bit for bit
     assert torch.equal(got, ep.expert_weight_grad(d, x, counts, out_dtype=out))
+
+
+@pytest.mark.parametrize("kind", ["random", "full", "one", "none"])
+@pytest.mark.parametrize("e, r, length, n, k", [
+    (1, 3, 700, 8, 8),        # few tiles, many rows
+    (3, 2, 1100, 88, 3544),
+    (2, 1, 1, 72, 64),
+    (9, 1, 130, 520, 1032),   # tiles for half of the card
+    (20, 3, 30, 1304, 1032),  # and for more than all of it
+])
+def test_weight_grad_of_all_sizes(e, r, length, n, k, kind):
+    g = gen(n)
+    counts = some_counts(g, e, r, length, kind)
+    mask = mask_of(counts, r * length)[..., None]
+    d = (randn(g, e, r * length, n) * 0.05).to(BF)
+    x = randn(g, e, r * length, k).to(BF)
+    d[~mask[..., 0]], x[~mask[..., 0]] = math.nan, math.nan
+    room = torch.full((e, n + 1, k + 8), 7.0, device="cuda")
+    got = ep.expert_weight_grad(d, x, counts, out=room[:, :n, :k])
+    d0 = torch.where(mask, d.double(), 0.0).transpose(1, 2).contiguous()
+    x0 = torch.where(mask, x.double(), 0.0)
+    want, size = torch.matmul(d0, x0), torch.matmul(d0.abs(), x0.abs())
+    close(got, want, want.abs() * STEP32 + size * r * length * STEP32,
+          "weight gradient")
+    assert (room[:, n:] == 7).all() and (room[:, :, k:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", ["random", "full", "one", "none"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("e, r, length, n, k, expected", [
+    (1, 2, 100, 8, 1000, None),    # few tiles, a long contraction
+    (2, 3, 60, 200, 72, 7),
+    (3, 1, 1, 64, 8, None),
+    (4, 1, 300, 1032, 136, None),  # tiles for half of the card
+    (40, 2, 40, 1032, 200, 40),    # few rows of many experts
+    (40, 2, 40, 1032, 200, 80),
+])
+def test_row_gradient_of_all_sizes(e, r, length, n, k, expected, dtype, kind):
+    g = gen(n + k)
+    counts = some_counts(g, e, r, length, kind)
+    mask = mask_of(counts, r * length)
+    x = randn(g, e, r * length, k).to(dtype)
+    x[~mask] = math.nan
+    w = (randn(g, e, k, n) * 0.05).to(dtype).transpose(1, 2)
+    y = torch.full((e, r * length, n), 7.0, dtype=dtype, device="cuda")
+    before = y.clone()
+    ep.expert_matmul(x, w, counts, out=y, expected_rows=expected)
+    x0 = torch.where(mask[..., None], x.double(), 0.0)
+    check_product(y, x0, w.double(), mask, before=before)
 
 
 def test_weight_grad_strides_and_two_dimensions():

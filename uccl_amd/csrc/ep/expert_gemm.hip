@@ -968,6 +968,59 @@ __device__ __forceinline__ void multiply_rows(
       joined[((i * NQ + j) * kRowWaves + wave) * 64 + lane] = acc[i][j];
 }
 
+// Valid rows of expert e up to and with each source, to `ends`; and all.
+__device__ __forceinline__ int count_rows(int* ends, SlotRows const& r,
+                                          int e) {
+  if (!r.counts) return r.length;
+  if (threadIdx.x < 64) {
+    int const lane = threadIdx.x;
+    int carry = 0;
+    for (int s0 = 0; s0 < r.sources; s0 += 64) {
+      int v = s0 + lane < r.sources
+                  ? min(max(r.counts[e * r.sources + s0 + lane], 0), r.length)
+                  : 0;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        int const o = __shfl_up(v, off);
+        if (lane >= off) v += o;
+      }
+      if (s0 + lane < r.sources) ends[s0 + lane] = carry + v;
+      carry += __shfl(v, 63);
+    }
+  }
+  __syncthreads();
+  return ends[r.sources - 1];
+}
+__device__ __forceinline__ int slot_at(int const* ends, SlotRows const& r,
+                                       int i) {
+  if (!r.counts) return i;
+  int begin = 0;
+  for (int s = 0; s < r.sources; ++s) {
+    int const end = ends[s];
+    if (i < end) return s * r.length + i - begin;
+    begin = end;
+  }
+  return 0;
+}
+
+// 4 results of consecutive p, the first `n` of them.
+template <Elem kOut>
+__device__ __forceinline__ void store4(char* at, f32x4 v, int n, bool wide) {
+  using T = OutType<kOut>;
+  if (wide && n >= 4) {
+    struct alignas(4 * sizeof(T)) Four {
+      T v[4];
+    } four;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) four.v[k] = static_cast<T>(v[k]);
+    *reinterpret_cast<Four*>(at) = four;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < n) reinterpret_cast<T*>(at)[k] = static_cast<T>(v[k]);
+  }
+}
+
 template <Elem kElem, Elem kOut, int TP>
 __global__ __launch_bounds__(kRowWaves * 64, 2) void k_expert_rows(
     GemmArgs a) {
@@ -978,40 +1031,9 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void k_expert_rows(
   __shared__ int ends[kMaxSlotCells];
   int const wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int const e = blockIdx.y, p0 = blockIdx.x * (16 * TP);
-  int const sources = a.rows.sources;
 
-  // valid rows up to and with each source
-  int valid = a.rows.length;
-  if (a.rows.counts) {
-    if (wave == 0) {
-      int carry = 0;
-      for (int s0 = 0; s0 < sources; s0 += 64) {
-        int v = s0 + lane < sources
-                    ? min(max(a.rows.counts[e * sources + s0 + lane], 0),
-                          a.rows.length)
-                    : 0;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          int const o = __shfl_up(v, off);
-          if (lane >= off) v += o;
-        }
-        if (s0 + lane < sources) ends[s0 + lane] = carry + v;
-        carry += __shfl(v, 63);
-      }
-    }
-    __syncthreads();
-    valid = ends[sources - 1];
-  }
-  auto slot = [&](int i) {
-    if (!a.rows.counts) return i;
-    int begin = 0;
-    for (int s = 0; s < sources; ++s) {
-      int const end = ends[s];
-      if (i < end) return s * a.rows.length + i - begin;
-      begin = end;
-    }
-    return 0;
-  };
+  int const valid = count_rows(ends, a.rows, e);
+  auto slot = [&](int i) { return slot_at(ends, a.rows, i); };
 
   char const* const pe = a.p + e * a.p_expert;
   char const* const qe = a.q + e * a.q_expert;
@@ -1061,20 +1083,184 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void k_expert_rows(
       if (q < valid && p < a.np) {
         char* const o = a.out + e * a.out_expert + slot(q) * a.out_row +
                         static_cast<int64_t>(p) * kOutSize;
-        using T = OutType<kOut>;
-        if (a.wide && p + 4 <= a.np) {
-          struct alignas(4 * kOutSize) Four {
-            T v[4];
-          } four;
+        store4<kOut>(o, sum, a.np - p, a.wide);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The same where P is turned (weights as they lie for the rows' gradient) or
+// both are (weight gradient), 16 bits: tiles of 64 x 64, whose 8 waves share
+// the contraction in steps of 64. Each wave turns its part of an operand in
+// its own piece of LDS, written from registers, so waves wait for nobody until
+// they join their sums. Bound by the length of the contraction. 3246 rows of 2
+// experts, weight gradient 56 x 72: 12 us.
+constexpr int kLongWaves = 8;
+
+template <Mode kMode, Elem kElem, Elem kOut>
+__global__ __launch_bounds__(kLongWaves * 64, 2) void k_expert_long(
+    GemmArgs a) {
+  constexpr bool kWGrad = kMode == Mode::kWeightGrad;
+  constexpr int kOutSize = kOut == Elem::kF32 ? 4 : 2;
+  constexpr int kSide = 64, kRowBytes = kSide * 2, kPiece = kSide * kRowBytes;
+  static_assert(kStep == 2 * kSide, "a step of a direct operand");
+  // pieces of the waves, P before Q; then their sums, 16 tiles a wave
+  __shared__ __attribute__((aligned(1024))) char lds[kLongWaves * 2 * kPiece];
+  __shared__ int ends[kMaxSlotCells];
+  f32x4* const joined = reinterpret_cast<f32x4*>(lds);
+  int const wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int const e = blockIdx.y, p0 = blockIdx.x * kSide;
+  int const valid = count_rows(ends, a.rows, e);
+  char const* const pe = a.p + e * a.p_expert;
+  char const* const qe = a.q + e * a.q_expert;
+  int const depth = kWGrad ? valid : a.depth;
+  int const steps = (depth + kSide - 1) / kSide;
+  int const begin = static_cast<int64_t>(steps) * wave / kLongWaves;
+  int const end = static_cast<int64_t>(steps) * (wave + 1) / kLongWaves;
+
+  // this lane's part of a turned operand: 16 bytes of 8 rows
+  int const row = lane >> 3, chunk = lane & 7;
+  int64_t const p_col = static_cast<int64_t>(min(p0 + chunk * 8, a.np - 8)) * 2;
+  char* const my_p = lds + wave * 2 * kPiece;
+  char* const my_q = my_p + kPiece;
+  int const put = row * kRowBytes + ((chunk ^ ((row & 3) << 2 & 7)) * 16);
+  // and of the reads that turn it
+  int const r = (lane >> 2) & 3, c = lane & 3;
+  int const turn = ((lane >> 4) * 8 + r) * kRowBytes;
+  uint32_t const get_lo = turn + ((c ^ (r << 2 & 7)) * 16);
+  uint32_t const get_hi = turn + (((c + 4) ^ (r << 2 & 7)) * 16);
+  auto turned = [&](char* piece, int i) {
+    uint32_t const at =
+        lds_addr(piece) + (i >> 1 ? get_hi : get_lo) + (i & 1) * 8;
+    i16x4 const v0 = lds_read_turned(at);
+    i16x4 const v1 = lds_read_turned(at + 4 * kRowBytes);
+    i16x4 const v2 = lds_read_turned(at + 32 * kRowBytes);
+    i16x4 const v3 = lds_read_turned(at + 36 * kRowBytes);
+    i32x4 const x = __builtin_bit_cast(
+        i32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+    i32x4 const y = __builtin_bit_cast(
+        i32x4, __builtin_shufflevector(v2, v3, 0, 1, 2, 3, 4, 5, 6, 7));
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+
+  int const q_end = kWGrad ? a.nq : valid;
+  for (int q0 = blockIdx.z * kSide; q0 < q_end; q0 += gridDim.z * kSide) {
+    int64_t const q_col =
+        kWGrad ? static_cast<int64_t>(min(q0 + chunk * 8, a.nq - 8)) * 2 : 0;
+    char const* q_at[4];
+    if constexpr (!kWGrad) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v) four.v[v] = static_cast<T>(sum[v]);
-          *reinterpret_cast<Four*>(o) = four;
-        } else {
+      for (int j = 0; j < 4; ++j)
+        q_at[j] = qe + static_cast<int64_t>(slot_at(
+                           ends, a.rows,
+                           min(q0 + j * 16 + (lane & 15), valid - 1))) *
+                           a.q_row;
+    }
+    // the source that this lane's next row of the contraction lies in
+    int seg = -1, seg_begin = 0, seg_end = 0;
+    i32x4 const zero = {0, 0, 0, 0};
+    struct Part {
+      i32x4 p[8];
+      i32x4 q[8];  // turned: 8 rows; direct: two halves of 4 tiles
+    };
+    auto load = [&](Part& t, int step) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (p + v < a.np)
-              reinterpret_cast<T*>(o)[v] = static_cast<T>(sum[v]);
+      for (int l = 0; l < 8; ++l) {
+        int const i = step * kSide + l * 8 + row;
+        t.p[l] = zero;
+        if constexpr (kWGrad) t.q[l] = zero;
+        if (i < depth) {
+          int64_t at = i;
+          if constexpr (kWGrad) {
+            if (a.rows.counts) {
+              while (i >= seg_end) {  // ends: the last end is `valid`
+                ++seg;
+                seg_begin = seg_end;
+                seg_end = ends[seg];
+              }
+              at = static_cast<int64_t>(seg) * a.rows.length + i - seg_begin;
+            }
+            t.q[l] = *reinterpret_cast<i32x4 const*>(qe + at * a.q_row + q_col);
+          }
+          t.p[l] = *reinterpret_cast<i32x4 const*>(pe + at * a.p_row + p_col);
         }
+      }
+      if constexpr (!kWGrad) {
+#pragma unroll
+        for (int l = 0; l < 8; ++l) {
+          int64_t const at = static_cast<int64_t>(step) * kStep +
+                             (lane >> 4) * 16 + (l & 1) * 64;
+          t.q[l] = at < static_cast<int64_t>(depth) * 2
+                       ? *reinterpret_cast<i32x4 const*>(q_at[l >> 1] + at)
+                       : zero;
+        }
+      }
+    };
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Part part;
+    if (begin < end) load(part, begin);
+    for (int step = begin; step < end; ++step) {
+      i32x8 pf[4], qf[4];
+#pragma unroll
+      for (int l = 0; l < 8; ++l) {
+        *reinterpret_cast<i32x4*>(my_p + l * 8 * kRowBytes + put) = part.p[l];
+        if constexpr (kWGrad)
+          *reinterpret_cast<i32x4*>(my_q + l * 8 * kRowBytes + put) = part.q[l];
+      }
+      if constexpr (!kWGrad) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          qf[j] = __builtin_shufflevector(part.q[2 * j], part.q[2 * j + 1], 0,
+                                          1, 2, 3, 4, 5, 6, 7);
+      }
+      if (step + 1 < end) load(part, step + 1);
+      // the lanes of this wave see each other's part
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pf[i] = turned(my_p, i);
+        if constexpr (kWGrad) qf[i] = turned(my_q, i);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[i][j] = mfma16<kElem>(half<0>(pf[i]), half<0>(qf[j]), acc[i][j]);
+          acc[i][j] = mfma16<kElem>(half<1>(pf[i]), half<1>(qf[j]), acc[i][j]);
+        }
+    }
+    __syncthreads();  // `joined` lies where the pieces do
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        joined[((i * 4 + j) * kLongWaves + wave) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    for (int t = wave; t < 16; t += kLongWaves) {
+      int const i = t >> 2, j = t & 3, m = lane & 15;
+      f32x4 sum = joined[t * kLongWaves * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < kLongWaves; ++w)
+        sum += joined[(t * kLongWaves + w) * 64 + lane];
+      int const p = p0 + (i >> 1) * 32 + (lane >> 4) * 8 + (i & 1) * 4;
+      int const q =
+          q0 + (kWGrad ? (j >> 1) * 32 + (m >> 2) * 8 + (j & 1) * 4 + (m & 3)
+                       : j * 16 + m);
+      if (q < q_end && p < a.np) {
+        int64_t const at = kWGrad ? q : slot_at(ends, a.rows, q);
+        store4<kOut>(a.out + e * a.out_expert + at * a.out_row +
+                         static_cast<int64_t>(p) * kOutSize,
+                     sum, a.np - p, a.wide);
       }
     }
     __syncthreads();
@@ -1122,6 +1308,13 @@ void launch_rows(GemmArgs const& a, int expected_rows, hipStream_t s) {
   k_expert_rows<kElem, kOut, TP><<<grid, kRowWaves * 64, 0, s>>>(a);
 }
 
+template <Mode kMode, Elem kElem, Elem kOut>
+void launch_long(GemmArgs const& a, int expected_rows, hipStream_t s) {
+  dim3 const grid((a.np + 63) / 64, a.rows.experts,
+                  std::min((expected_rows + 63) / 64, 1024));
+  k_expert_long<kMode, kElem, kOut><<<grid, kLongWaves * 64, 0, s>>>(a);
+}
+
 // Which kernel, by the rows that an expert is expected to have and the tiles
 // that this makes. Measured in us:
 //   32 experts, 4096 x 7168, 8 bits      rows:   8    16    32    64   128
@@ -1142,6 +1335,17 @@ void launch_rows(GemmArgs const& a, int expected_rows, hipStream_t s) {
 //     tiles of 128 x 128                  17.2
 //     tiles of 256 x 128                  12.5
 //     tiles of 256 x 256                  15.8
+//     k_expert_long                       46.5
+//   the same, n x k (experts, rows)  56 x 72   512 x 512   512 x 512  88 x 3544
+//                                   (2, 1623)   (8, 139)   (8, 2500) (3, 3345)
+//     tiles of 256 x 128               32.6       10.3        51.7       66.4
+//     k_expert_long                    11.9       12.5        43.3       44.1
+//   row gradient, 128 rows           512 x 1024 of 4 / 8 experts
+//     tiles of 128 x 128               14.8 / 15.0
+//     k_expert_long                    10.3 / 10.5
+//   row gradient, 6 rows of 32 experts, 1024 x 512
+//     tiles of 256 x 64                10.5
+//     k_expert_long                    14.2
 template <Mode kMode, Elem kElem, Elem kOut>
 void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
   auto tiles = [&](int p, int q) {
@@ -1157,6 +1361,12 @@ void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
         launch_rows<kElem, kOut, 1>(a, expected_rows, s);
       return;
     }
+  }
+  if constexpr (kMode != Mode::kProduct) {
+    bool const many_rows = kMode == Mode::kWeightGrad &&
+                           a.rows.sources * a.rows.length > 2048;
+    if (tiles(64, 64) <= (many_rows ? 2 : 1) * cus)
+      return launch_long<kMode, kElem, kOut>(a, expected_rows, s);
   }
   if constexpr (kElem == Elem::kF8) {
     if (!a.near)

@@ -159,7 +159,7 @@ def expert_weight_grad(grad_out: torch.Tensor, x: torch.Tensor,
     gradient of expert_matmul's weights, [E, N, K]. grad_out [E, slots, N] and
     x [E, slots, K] are bfloat16 or float16 with N and K multiples of 8; out
     has their dtype, or ``out_dtype`` (bfloat16, float16, float32). Sums are
-    held in 32 bits and taken in the order of the rows. An expert without
+    held in 32 bits and taken in a fixed order. An expert without
     valid rows gets zeros."""
     C = _native(grad_out=grad_out, x=x, out=out)
     if out is None:

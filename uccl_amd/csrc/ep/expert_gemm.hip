@@ -174,7 +174,6 @@ struct GemmArgs {
   int nq;     // extent of q (weight gradient only; else the valid rows)
   int depth;  // contraction in elements (product only)
   bool near;  // a lane's addresses in a stage lie within 32 bits
-  bool wide;  // 8 results of a row can be stored together
   char const* q_scales;
   char const* p_scales;
   int64_t qs_expert, qs_row, ps_expert, ps_row;  // bytes
@@ -205,21 +204,15 @@ using OutType = std::conditional_t<
     kOut == Elem::kF32, float,
     std::conditional_t<kOut == Elem::kBF16, __bf16, _Float16>>;
 
-// Store 8 results of a row, at a 16-byte boundary; or the first n of them.
+// Store 8 results of a row, or the first n of them. 16 bytes at a time at any
+// address: this target allows it, and a row of odd length starts anywhere.
 template <Elem kOut>
 __device__ __forceinline__ void store8(char* at, f32x4 a, f32x4 b) {
   using T = OutType<kOut>;
-  struct alignas(16) Pack {
-    T v[16 / sizeof(T)];
-  };
-  Pack pack[sizeof(T) / 2];
+  T v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    pack[j * sizeof(T) / 16].v[j % (16 / sizeof(T))] =
-        static_cast<T>(j < 4 ? a[j % 4] : b[j % 4]);
-#pragma unroll
-  for (unsigned j = 0; j < sizeof(T) / 2; ++j)
-    reinterpret_cast<Pack*>(at)[j] = pack[j];
+  for (int j = 0; j < 8; ++j) v[j] = static_cast<T>(j < 4 ? a[j % 4] : b[j % 4]);
+  __builtin_memcpy(at, v, sizeof(v));
 }
 template <Elem kOut>
 __device__ __forceinline__ void store_few(char* at, f32x4 a, f32x4 b, int n) {
@@ -833,7 +826,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
         return wq * RQ + (j >> 1) * 32 + ((lane & 15) >> 2) * 8 +
                (j & 1) * 4 + (lane & 3);
     };
-    if (a.wide && done.p0 + BP <= a.np) {
+    if (done.p0 + BP <= a.np) {
       // All columns are inside, and a row behind the last holds what a row
       // inside does, which it stores again: so every lane stores, and the
       // number of stores in flight is known.
@@ -864,7 +857,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
 #pragma unroll
         for (int i = 0; i < TP; i += 2) {
           int const n = a.np - (out_p + i * 16);
-          if (n >= 8 && a.wide)
+          if (n >= 8)
             store8<kOut>(o + i * 16 * kOutSize, acc[i][j], acc[i + 1][j]);
           else
             store_few<kOut>(o + i * 16 * kOutSize, acc[i][j], acc[i + 1][j],
@@ -1005,15 +998,13 @@ __device__ __forceinline__ int slot_at(int const* ends, SlotRows const& r,
 
 // 4 results of consecutive p, the first `n` of them.
 template <Elem kOut>
-__device__ __forceinline__ void store4(char* at, f32x4 v, int n, bool wide) {
+__device__ __forceinline__ void store4(char* at, f32x4 v, int n) {
   using T = OutType<kOut>;
-  if (wide && n >= 4) {
-    struct alignas(4 * sizeof(T)) Four {
-      T v[4];
-    } four;
+  if (n >= 4) {
+    T four[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) four.v[k] = static_cast<T>(v[k]);
-    *reinterpret_cast<Four*>(at) = four;
+    for (int k = 0; k < 4; ++k) four[k] = static_cast<T>(v[k]);
+    __builtin_memcpy(at, four, sizeof(four));
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -1083,7 +1074,7 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void k_expert_rows(
       if (q < valid && p < a.np) {
         char* const o = a.out + e * a.out_expert + slot(q) * a.out_row +
                         static_cast<int64_t>(p) * kOutSize;
-        store4<kOut>(o, sum, a.np - p, a.wide);
+        store4<kOut>(o, sum, a.np - p);
       }
     }
     __syncthreads();
@@ -1260,7 +1251,7 @@ __global__ __launch_bounds__(kLongWaves * 64, 2) void k_expert_long(
         int64_t const at = kWGrad ? q : slot_at(ends, a.rows, q);
         store4<kOut>(a.out + e * a.out_expert + at * a.out_row +
                          static_cast<int64_t>(p) * kOutSize,
-                     sum, a.np - p, a.wide);
+                     sum, a.np - p);
       }
     }
     __syncthreads();
@@ -1280,11 +1271,6 @@ int compute_units() {
 bool lies_near(GemmArgs const& a, int64_t p_span, int64_t q_span) {
   constexpr int64_t kEnd = (int64_t{1} << 32) - 16384;
   return p_span * a.p_row < kEnd && q_span * a.q_row < kEnd;
-}
-
-bool stores_wide(GemmArgs const& a) {
-  return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row % 16 == 0 &&
-         a.out_expert % 16 == 0;
 }
 
 template <Mode kMode, Elem kElem, Elem kOut, int BP, int BQ, int WP, int WQ,
@@ -1415,7 +1401,6 @@ void launch_expert_matmul(MatmulArgs const& m, hipStream_t s) {
   a.np = m.n;
   int64_t const slots = static_cast<int64_t>(m.rows.sources) * m.rows.length;
   a.near = lies_near(a, 256, slots);
-  a.wide = stores_wide(a);
   a.depth = m.k;
   if (m.elem == Elem::kF8) {
     a.p_scales = static_cast<char const*>(m.w_scales.p);
@@ -1456,7 +1441,6 @@ void launch_expert_weight_grad(WeightGradArgs const& w, hipStream_t s) {
   a.np = w.k;
   int64_t const slots = static_cast<int64_t>(w.rows.sources) * w.rows.length;
   a.near = lies_near(a, slots, slots);
-  a.wide = stores_wide(a);
   a.nq = w.n;
   if (w.elem == Elem::kBF16)
     by_out<Mode::kWeightGrad, Elem::kBF16>(a, w.out_elem, w.n, s);

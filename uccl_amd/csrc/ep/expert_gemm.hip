@@ -1308,6 +1308,11 @@ void launch_long(GemmArgs const& a, int expected_rows, hipStream_t s) {
 //     tiles of 256 x 64                                    172   215   309
 //     tiles of 256 x 128                                   190   197   256
 //     tiles of 256 x 256                       252   255   253   266   271
+//   the same, rows on average, experts     10    24    32    48    94   128
+//   of unlike popularity
+//     tiles of 256 x 64                     159   169   209   201   251   303
+//     tiles of 256 x 128                    180   170   172   177   238   247
+//     tiles of 256 x 256                    265   253   260   250   265   258
 //   1 expert, 7168 x 2048, 8 bits        rows:   1    16    64
 //     k_expert_rows                            5.5   7.6  16.4
 //     tiles of 128 x 128                      20.0  20.1  20.4
@@ -1361,7 +1366,7 @@ void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
   if constexpr (kMode != Mode::kWeightGrad) {
     if (tiles(128, 128) <= cus / 2)
       return launch_tiles<kMode, kElem, kOut, 128, 128, 2, 2>(a, 2, s);
-    if (expected_rows <= 48)
+    if (expected_rows <= 24)
       return launch_tiles<kMode, kElem, kOut, 256, 64, 4, 1>(a, 1, s);
     if (expected_rows <= 96)
       return launch_tiles<kMode, kElem, kOut, 256, 128, 4, 2>(a, 1, s);

@@ -70,7 +70,7 @@ __device__ const int4 zero_page = {0, 0, 0, 0};
 // it does not cut the block that the compiler schedules.
 #define LDS_LOAD_GROUP(loads, last, ...)                                      \
   asm volatile("s_cmp_eq_u32 %1, 0\n\ts_cbranch_scc1 1f\n\t"                  \
-               "s_mov_b32 m0, %2\n\ts_nop 0\n\t" loads "\n1:"               \
+               "s_mov_b32 m0, %2\n\ts_nop 0\n\t" loads "\n1:"                 \
                :                                                              \
                : "s"(base), "s"(on), "s"(lds), "n"(last), __VA_ARGS__         \
                : "memory", "m0", "scc")
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
     }
   };
   // Loads of stage `step`: parts 0 and 1 are P, 2 and 3 the halves of Q.
-  // A wave's first loads of a stage are counted on to be done in this order.
+  // Barriers count on this order.
   auto load_near = [&](auto n, int on, int step)
                        __attribute__((always_inline)) {
     constexpr int part = decltype(n)::value;

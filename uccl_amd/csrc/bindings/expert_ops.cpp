@@ -283,7 +283,7 @@ void route_grad(at::Tensor grad_weights, at::Tensor logits, at::Tensor idx,
 
 void expert_matmul(at::Tensor x, at::Tensor w, OptTensor counts,
                    OptTensor x_scales, OptTensor w_scales, at::Tensor out,
-                   int64_t expected_rows) {
+                   int64_t expected_rows, bool precise) {
   check_slots(x, "x");
   check_on(w, x, "w");
   check_on(out, x, "out");
@@ -319,9 +319,11 @@ void expert_matmul(at::Tensor x, at::Tensor w, OptTensor counts,
                 "uccl_amd: 8-bit products need k % 128 == 0, got ", k);
     TORCH_CHECK(n == 1 || w.stride(1) < (int64_t(1) << 24),
                 "uccl_amd: rows of 8-bit weights are less than 16 MiB apart");
-    TORCH_CHECK(a.out_elem != Elem::kF32,
+    TORCH_CHECK(a.out_elem != Elem::kF32 || precise,
                 "uccl_amd: 8-bit products give bfloat16 or float16: the 8-bit "
-                "matrix unit does not keep the precision of float32");
+                "matrix unit does not keep the precision of float32 "
+                "(precise=True does without it)");
+    a.precise = precise;
     for (auto const& [t, name] : {std::pair(*x_scales, "x_scales"),
                                   std::pair(*w_scales, "w_scales")}) {
       check_on(t, x, name);
@@ -336,6 +338,8 @@ void expert_matmul(at::Tensor x, at::Tensor w, OptTensor counts,
   } else {
     TORCH_CHECK(!x_scales && !w_scales,
                 "uccl_amd: scales belong to 8-bit operands");
+    TORCH_CHECK(!precise, "uccl_amd: precise belongs to 8-bit operands; sums "
+                "of 16-bit ones are held in 32 bits");
     TORCH_CHECK(k % 8 == 0,
                 "uccl_amd: 16-bit products need k % 8 == 0, got ", k);
   }

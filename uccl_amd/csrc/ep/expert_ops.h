@@ -70,6 +70,7 @@ struct MatmulArgs {
   // k/128], dense in their last dimension
   Mat x_scales, w_scales;
   int expected_rows;  // rows an expert is expected to have; picks the tile
+  bool precise;  // 8-bit only: sums of 32 bits, and any out_elem
 };
 void launch_expert_matmul(MatmulArgs const& a, hipStream_t s);
 

@@ -1,8 +1,8 @@
 // Gated activation between two expert products, and its gradient.
 //
 //   v = silu(a) b, a the first half of a row's columns, b the second
-//   to 8 bits: s = max|v| / 448 over each 128 columns (1 if all are 0),
-//              q = the e4m3 value nearest to v / s, ties to even
+//   to 8 bits: s = max|v| / 448 over each 128 columns (1 where that is 0 as a
+//              float), q = the e4m3 value nearest to v / s, ties to even
 //   gradient: da = g b sig(a) (1 + a (1 - sig(a))), db = g silu(a)
 //
 // Every value is read and written once, 16 bytes a lane and load; a wave takes
@@ -361,10 +361,10 @@ __global__ __launch_bounds__(256) void k_swiglu_quant(SwigluArgs a) {
       // the quotient by 448, rounded once: a product with 1 / 448, corrected
       double q = largest * (1.0 / 448.0);
       q = fma(fma(-448.0, q, largest), 1.0 / 448.0, q);
-      scale[k] =
-          largest > 0.0
-              ? static_cast<float>(largest < INFINITY ? q : largest)
-              : 1.f;
+      scale[k] = static_cast<float>(largest < INFINITY ? q : largest);
+      // also where the largest is not 0 but its 448th part rounds to 0: the
+      // group's values then are 0, not quotients by 0
+      if (!(scale[k] > 0.f)) scale[k] = 1.f;
       float const inverse = __builtin_amdgcn_rcpf(scale[k]);
       unsigned differ[2];
 #pragma unroll

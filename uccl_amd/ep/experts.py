@@ -190,9 +190,10 @@ def expert_swiglu(h: torch.Tensor, counts: Optional[torch.Tensor] = None, *,
 
     Returns [E, slots, I] in h's dtype. With ``quantize`` (I a multiple of
     128) returns (values float8_e4m3fn, scales float32 [E, slots, I/128]) for
-    an 8-bit expert_matmul: scale = max |v| / 448 over each 128 columns (1 if
-    all are 0), values the nearest to v / scale, ties to even, decided as if v
-    were exact."""
+    an 8-bit expert_matmul: scale = max |v| / 448 over each 128 columns, or 1
+    where that is 0 as a float32; values the nearest to v / scale, ties to
+    even, decided as if v were exact. A NaN stays NaN and does not count for
+    its scale; an infinite v makes its scale infinite and itself NaN."""
     C = _native(h=h, out=out, out_scales=out_scales)
     cols = h.shape[-1] // 2
     if out is None:

@@ -1,6 +1,9 @@
 """The gated activation where its values leave the ordinary range: closed
 gates, scales below the smallest float, infinities and NaN, against the
 formulas in 64 bits on the CPU.
+
+Tolerances in 16 bits as for ordinary values: the half step of the type, an
+exponential good to 2 units and six more operations in 32 bits.
 """
 
 import math
@@ -16,6 +19,7 @@ if not torch.cuda.is_available():
 import uccl_amd.ep as ep  # noqa: E402
 
 F8, BF, HF = torch.float8_e4m3fn, torch.bfloat16, torch.float16
+STEP32 = 2.0 ** -23
 
 
 def swiglu(a, b):
@@ -92,3 +96,59 @@ def test_swiglu_8bit_of_infinities_and_nan(dtype):
         a[row, 37], b[row, 37] = x, y
     a[8] = nan
     check_quantized(a, b, dtype)
+
+
+def same_kind(got, want, tol):
+    """The same NaN and infinities, other values within tol."""
+    assert torch.equal(got.isnan(), want.isnan()), (got, want)
+    far = want.isinf()
+    assert torch.equal(got[far], want[far]), (got[far], want[far])
+    fine = want.isfinite()
+    assert ((got - want).abs() <= tol)[fine].all(), (got[fine], want[fine])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_swiglu_and_gradient_of_infinities_and_nan(dtype):
+    """At a gate of +inf the result and the second half's gradient are
+    infinite. The formulas leave 0 * inf, NaN, for the first half's gradient
+    there, and for all three at -inf."""
+    inf, nan = math.inf, math.nan
+    special = [inf, -inf, nan, 1.0, -3.0, 50.0, -20.0, 0.0]
+    a, b = torch.meshgrid(torch.tensor(special),
+                          torch.tensor([inf, -inf, nan, 2.0, -0.5, 1.0, -1.0,
+                                        0.0]), indexing="ij")
+    a, b = a.reshape(1, -1).to(dtype), b.reshape(1, -1).to(dtype)
+    d = torch.linspace(-2, 3, 64).to(dtype)[None]
+    h = torch.cat([a, b], -1)
+    out = ep.expert_swiglu(h.cuda()).cpu().double()
+    grad = ep.expert_swiglu_grad(d.cuda(), h.cuda()).cpu().double()
+
+    u = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * u * 2
+    want = swiglu(a, b)
+    same_kind(out, want, want.abs() * (u + 8 * STEP32) + tiny)
+    x, y, g = a.double(), b.double(), d.double()
+    sig = torch.sigmoid(x)
+    da = g * y * sig * (1 + x * (1 - sig))
+    db = g * x * sig
+    terms = torch.cat([(g * y).abs() * sig * (1 + x.abs()), db.abs()], -1)
+    want = torch.cat([da, db], -1)
+    same_kind(grad, want, want.abs() * u + terms * 12 * STEP32 + tiny)
+
+
+def test_swiglu_of_gates_at_the_ends_of_the_type():
+    """Finite gates whose exponential underflows or is 1: no NaN arises."""
+    big = torch.finfo(BF).max
+    a = torch.tensor([[big, -big, 1e30, -1e30, 300.0, -300.0, 1000.0, -1000.0]])
+    b = torch.tensor([[1e-30, 2.0, -1e-10, -2.0, 1.0, 1.0, 0.0, 0.0]])
+    a, b = a.to(BF), b.to(BF)
+    h = torch.cat([a, b], -1)
+    out = ep.expert_swiglu(h.cuda()).cpu().double()
+    want = swiglu(a, b)
+    same_kind(out, want, want.abs() * (2.0 ** -8 + 8 * STEP32) + 1e-38)
+    d = torch.ones(1, 8, dtype=BF)
+    grad = ep.expert_swiglu_grad(d.cuda(), h.cuda()).cpu().double()
+    sig = torch.sigmoid(a.double())
+    da = b.double() * sig * (1 + a.double() * (1 - sig))
+    want = torch.cat([da, a.double() * sig], -1)
+    same_kind(grad, want, want.abs() * (2.0 ** -8 + 12 * STEP32) + 1e-38)

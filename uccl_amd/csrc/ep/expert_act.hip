@@ -145,7 +145,10 @@ __device__ __forceinline__ void store8(char* row, int col, f32x8 v) {
 __device__ __forceinline__ float half_exp(float a) {
   // log2(e) / 2, in two parts
   constexpr float kHigh = 0.72134752f, kLow = 9.629815e-9f;
-  float const x = -fabsf(a);
+  // Beyond -1000 the exponential is 0 as well, and an infinite a would leave
+  // inf - inf in the lost part. (A NaN is lost here, but every result has a
+  // as a factor, too.)
+  float const x = fmaxf(-fabsf(a), -1000.f);
   float const h = x * kHigh;
   float const l = fmaf(x, kLow, fmaf(x, kHigh, -h));
   float const e = __builtin_amdgcn_exp2f(h);

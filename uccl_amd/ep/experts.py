@@ -186,7 +186,8 @@ def expert_swiglu(h: torch.Tensor, counts: Optional[torch.Tensor] = None, *,
                   out: Optional[torch.Tensor] = None,
                   out_scales: Optional[torch.Tensor] = None):
     """silu(a) * b for the valid rows of h [E, slots, 2 * I] (bfloat16 or
-    float16), a the first I columns and b the others; I a multiple of 8.
+    float16), a the first I columns and b the others; I a multiple of 8. A gate
+    a of +inf gives +-inf, one of -inf NaN, as a * sigmoid(a) * b does.
 
     Returns [E, slots, I] in h's dtype. With ``quantize`` (I a multiple of
     128) returns (values float8_e4m3fn, scales float32 [E, slots, I/128]) for
@@ -216,7 +217,8 @@ def expert_swiglu_grad(grad_out: torch.Tensor, h: torch.Tensor,
                        counts: Optional[torch.Tensor] = None, *,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of expert_swiglu's h, [E, slots, 2 * I] in its dtype, from
-    grad_out [E, slots, I] of the same dtype."""
+    grad_out [E, slots, I] of the same dtype. At an infinite gate the first
+    half's is NaN, as sigmoid(a) * (1 + a * (1 - sigmoid(a))) is."""
     C = _native(grad_out=grad_out, h=h, out=out)
     if out is None:
         out = torch.empty(h.shape, dtype=h.dtype, device=h.device)

@@ -26,7 +26,8 @@ boundaries, which sets the multiples of columns that the functions name.
 Nothing here records an autograd graph: each operator with a gradient has its
 own function for it, and an operand that requires grad is refused while grad
 mode is on, so that a gradient is not lost silently (call it under
-``torch.no_grad()``, from an ``autograd.Function``, or with ``.detach()``).
+``torch.no_grad()``, from an ``autograd.Function``, or with ``.detach()``). One
+that carries a forward-mode derivative is refused as well.
 """
 
 from __future__ import annotations
@@ -34,6 +35,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 
 def _native(**operands):
@@ -46,6 +48,15 @@ def _native(**operands):
                     f"uccl_amd: {name} requires grad, and this operator "
                     "records no autograd graph; call it under torch.no_grad() "
                     "and take the gradient from its *_grad function")
+    # inside a dual_level(), and whatever grad mode says; a Function's forward
+    # has them off
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for name, t in operands.items():
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(
+                    f"uccl_amd: {name} carries a forward-mode derivative, "
+                    "which this operator would drop; take the primal with "
+                    "torch.autograd.forward_ad.unpack_dual")
     return _load_native(required=True)
 
 

@@ -95,3 +95,56 @@ def test_an_autograd_function_may_call_them_in_forward_mode():
     plain = torch.zeros(2, 8, 16, dtype=BF)
     with forward_ad.dual_level():
         passes(Gate.apply, forward_ad.make_dual(plain, torch.ones_like(plain)))
+
+
+# --- results inside a larger tensor ----------------------------------------
+
+def test_results_may_lie_between_the_columns_of_operands():
+    room = torch.zeros(2, 6, 96, dtype=BF)
+    h, out, grad = room[..., :32], room[..., 32:48], room[..., 48:80]
+    w = torch.zeros(2, 16, 32, dtype=BF)
+    passes(ep.expert_swiglu, h, out=out)
+    passes(ep.expert_swiglu_grad, out, h, out=grad)
+    passes(ep.expert_swiglu_grad, room[..., 80:], grad, out=h)
+    passes(ep.expert_matmul, h, w, out=out)
+    passes(ep.expert_matmul, grad, w, out=out)
+    passes(ep.expert_matmul, h[:, :1], w, out=out[:, :1])
+    # weights read turned, between the columns of their gradient
+    both = torch.zeros(2, 16, 64, dtype=BF)
+    passes(ep.expert_weight_grad, room[..., 32:48], h, out=both[..., :32])
+    passes(ep.expert_matmul, out.contiguous(), both[..., :32].transpose(1, 2),
+           out=torch.zeros(2, 6, 32, dtype=BF))
+    # one row of 6, next to each other
+    flat = torch.zeros(6 * 48, dtype=BF)
+    passes(ep.expert_swiglu, flat[:192].view(1, 6, 32),
+           out=flat[192:].view(1, 6, 16))
+
+
+def test_results_that_share_an_element_with_an_operand_are_refused():
+    room = torch.zeros(2, 6, 96, dtype=BF)
+    h = room[..., :32]
+    w = torch.zeros(2, 16, 32, dtype=BF)
+    for first in (0, 8, 16, 24):
+        refused("overlaps", ep.expert_swiglu, h, out=room[..., first:first + 16])
+        refused("overlaps", ep.expert_matmul, h, w,
+                out=room[..., first:first + 16])
+    refused("overlaps", ep.expert_matmul, h, w, out=room[..., 31:47])
+    passes(ep.expert_matmul, h, w, out=room[..., 32:48])
+    # columns that a row's end wraps into
+    line = torch.zeros(2 * 6 * 48 + 48, dtype=BF)
+    x = line[40:].as_strided((2, 6, 32), (6 * 48, 48, 1))
+    refused("overlaps", ep.expert_matmul, x, w,
+            out=line.as_strided((2, 6, 16), (6 * 48, 48, 1), 16))
+    passes(ep.expert_matmul, x, w,
+           out=line.as_strided((2, 6, 16), (6 * 48, 48, 1), 24))
+    # another pitch, so that some rows meet
+    refused("overlaps", ep.expert_matmul, h, w,
+            out=room.view(-1).as_strided((2, 6, 16), (6 * 80, 80, 1), 32))
+    # rows shared by all experts
+    one = torch.zeros(6, 48, dtype=BF)
+    refused("overlaps", ep.expert_matmul, one[:, :32].expand(1, 6, 32), w[:1],
+            out=one[:, 31:47].unsqueeze(0))
+    # 8-bit values and their scales in one place
+    h8, q = torch.zeros(1, 6, 256, dtype=BF), torch.zeros(1, 6, 128).to(F8)
+    refused("out_scales overlaps", ep.expert_swiglu, h8, quantize=True, out=q,
+            out_scales=q.view(-1)[:24].view(torch.float32).view(1, 6, 1))

@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <numeric>
 #include <vector>
 
 #include "../ep/expert_ops.h"
@@ -75,8 +76,38 @@ int64_t span_of(at::Tensor const& t) {
   return (last + 1) * t.element_size();
 }
 
-// A result: no two elements share memory, and none lies between the first
-// and last byte of an operand.
+// Whether no element of `a` shares memory with one of `b`, as far as their
+// spans or the columns of a common pitch tell.
+bool lie_apart(at::Tensor const& a, at::Tensor const& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  auto const begin_a = reinterpret_cast<uintptr_t>(a.data_ptr());
+  auto const begin_b = reinterpret_cast<uintptr_t>(b.data_ptr());
+  if (begin_a + span_of(a) <= begin_b || begin_b + span_of(b) <= begin_a)
+    return true;
+  // Rows of contiguous elements, all of which start at multiples of `pitch`
+  // bytes from the tensor's first.
+  int64_t pitch = 0;
+  auto row_of = [&](at::Tensor const& t) {
+    int64_t row = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      if (t.size(d) <= 1) continue;
+      if (t.stride(d) == 1 && row == 0)
+        row = t.size(d) * t.element_size();
+      else
+        pitch = std::gcd(pitch, t.stride(d) * t.element_size());
+    }
+    return row ? row : t.element_size();
+  };
+  int64_t const row_a = row_of(a), row_b = row_of(b);
+  if (pitch == 0) return false;
+  // where rows of b start behind those of a
+  auto const ahead = static_cast<int64_t>(
+      begin_b >= begin_a ? (begin_b - begin_a) % pitch
+                         : (pitch - (begin_a - begin_b) % pitch) % pitch);
+  return row_a <= ahead && ahead + row_b <= pitch;
+}
+
+// A result: no two elements share memory, and none shares it with an operand.
 void check_result(at::Tensor const& out, char const* name,
                   std::vector<at::Tensor> const& operands) {
   std::vector<std::pair<int64_t, int64_t>> dims;
@@ -89,14 +120,8 @@ void check_result(at::Tensor const& out, char const* name,
                 " share memory (strides ", out.strides(), ")");
     extent += stride * (size - 1);
   }
-  auto const begin = reinterpret_cast<uintptr_t>(out.data_ptr());
-  auto const end = begin + span_of(out);
-  for (auto const& t : operands) {
-    auto const b = reinterpret_cast<uintptr_t>(t.data_ptr());
-    TORCH_CHECK(end <= b || b + span_of(t) <= begin || span_of(t) == 0 ||
-                    span_of(out) == 0,
-                "uccl_amd: ", name, " overlaps an operand");
-  }
+  for (auto const& t : operands)
+    TORCH_CHECK(lie_apart(out, t), "uccl_amd: ", name, " overlaps an operand");
 }
 
 // [experts, rows, cols] with contiguous columns whose rows start at 16-byte

@@ -148,3 +148,22 @@ def test_results_that_share_an_element_with_an_operand_are_refused():
     h8, q = torch.zeros(1, 6, 256, dtype=BF), torch.zeros(1, 6, 128).to(F8)
     refused("out_scales overlaps", ep.expert_swiglu, h8, quantize=True, out=q,
             out_scales=q.view(-1)[:24].view(torch.float32).view(1, 6, 1))
+
+
+def test_results_over_the_counts_are_refused():
+    """Blocks read the counts while others already write results."""
+    out = torch.zeros(2, 6, 16, dtype=BF)
+    counts = out.view(torch.int32).view(-1)[8:12].view(2, 2)
+    x, w = torch.zeros(2, 6, 32, dtype=BF), torch.zeros(2, 16, 32, dtype=BF)
+    refused("out overlaps", ep.expert_matmul, x, w, counts, out=out)
+    refused("out overlaps", ep.expert_swiglu, x, counts, out=out)
+    refused("out overlaps", ep.expert_swiglu_grad, torch.zeros_like(out[..., :8])
+            .contiguous(), x[..., :16].contiguous(), counts, out=out)
+    dw = torch.zeros(2, 8, 32, dtype=BF)
+    refused("out overlaps", ep.expert_weight_grad, x[..., :8].contiguous(), x,
+            dw.view(torch.int32).view(-1)[:4].view(2, 2), out=dw)
+    scales = torch.zeros(2, 6, 1)
+    refused("out_scales overlaps", ep.expert_swiglu,
+            torch.zeros(2, 6, 256, dtype=BF),
+            scales.view(torch.int32).view(-1)[:4].view(2, 2), quantize=True,
+            out_scales=scales)

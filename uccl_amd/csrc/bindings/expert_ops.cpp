@@ -107,9 +107,11 @@ bool lie_apart(at::Tensor const& a, at::Tensor const& b) {
   return row_a <= ahead && ahead + row_b <= pitch;
 }
 
-// A result: no two elements share memory, and none shares it with an operand.
+// A result: no two elements share memory, and none shares it with an operand
+// or with the counts.
 void check_result(at::Tensor const& out, char const* name,
-                  std::vector<at::Tensor> const& operands) {
+                  std::vector<at::Tensor> const& operands,
+                  OptTensor const& counts = {}) {
   std::vector<std::pair<int64_t, int64_t>> dims;
   for (int64_t d = 0; d < out.dim(); ++d)
     if (out.size(d) > 1) dims.emplace_back(out.stride(d), out.size(d));
@@ -122,6 +124,8 @@ void check_result(at::Tensor const& out, char const* name,
   }
   for (auto const& t : operands)
     TORCH_CHECK(lie_apart(out, t), "uccl_amd: ", name, " overlaps an operand");
+  TORCH_CHECK(!counts || lie_apart(out, *counts), "uccl_amd: ", name,
+              " overlaps the counts");
 }
 
 // [experts, rows, cols] with contiguous columns whose rows start at 16-byte
@@ -380,7 +384,7 @@ void expert_matmul(at::Tensor x, at::Tensor w, OptTensor counts,
     a.w = mat_of(w, "w");
   }
   a.out = mat_of(out, "out", out.element_size());
-  check_result(out, "out", operands);
+  check_result(out, "out", operands, counts);
   a.expected_rows =
       static_cast<int>(expected_rows ? std::min(expected_rows, slots) : slots);
   check_gpu(x, "x");
@@ -420,7 +424,7 @@ void expert_weight_grad(at::Tensor grad, at::Tensor x, OptTensor counts,
   a.out_elem = elem_of(out, "out");
   TORCH_CHECK(a.out_elem != Elem::kF8, "uccl_amd: out has unsupported dtype ",
               out.scalar_type());
-  check_result(out, "out", {grad, x});
+  check_result(out, "out", {grad, x}, counts);
   check_gpu(x, "x");
   c10::DeviceGuard guard(x.device());
   ep::launch_expert_weight_grad(a, stream_of(x));
@@ -459,14 +463,14 @@ void expert_swiglu(at::Tensor h, OptTensor counts, at::Tensor out,
                 scales->scalar_type());
     check_shape(*scales, {h.size(0), h.size(1), cols / 128}, "out_scales");
     a.scales = mat_of(*scales, "out_scales", 4);
-    check_result(*scales, "out_scales", {h, out});
+    check_result(*scales, "out_scales", {h, out}, counts);
   } else {
     TORCH_CHECK(out.scalar_type() == h.scalar_type(),
                 "uccl_amd: out must have the dtype of h, got ",
                 out.scalar_type());
   }
   a.out = mat_of(out, "out");
-  check_result(out, "out", operands);
+  check_result(out, "out", operands, counts);
   check_gpu(h, "h");
   if (h.size(1) == 0) return;
   c10::DeviceGuard guard(h.device());
@@ -497,7 +501,7 @@ void expert_swiglu_grad(at::Tensor grad, at::Tensor h, OptTensor counts,
   a.out = mat_of(out, "out");
   a.cols = static_cast<int>(cols);
   a.elem = elem_of(h, "h");
-  check_result(out, "out", {h, grad});
+  check_result(out, "out", {h, grad}, counts);
   check_gpu(h, "h");
   if (h.size(1) == 0) return;
   c10::DeviceGuard guard(h.device());

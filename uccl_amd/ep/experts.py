@@ -19,6 +19,8 @@ keep their values, in a fresh one they are undefined. ``counts=None``: all rows
 are valid; counts [experts] stands for one source (so the sums over ranks that
 ``deep_ep_compat`` returns fit only where there is one rank). Two-dimensional
 operands are those of a single expert. At most 1024 experts and 2048 counts.
+A result shares no memory with an operand or the counts; it may lie between an
+operand's columns in a larger tensor.
 
 Every call is enqueued on the current stream of its operands' device and may be
 captured into a graph. Operands lie on one device; rows start at 16-byte

@@ -46,12 +46,18 @@ class _Handle:
     """Dispatch handle: carries the routing (topk_idx) plus the plan
     generation so a later dispatch with the same handle can replay the
     cached compaction lists (DeepEP cached-handle mode,
-    reference ep/src/intranode.cu:150 cached_notify_dispatch)."""
+    reference ep/src/intranode.cu:150 cached_notify_dispatch).
 
-    def __init__(self, topk_idx, num_tokens, plan_gen):
+    recv_counts (low-latency dispatch): [local experts, ranks] int32 on the
+    GPU, how many rows of each expert came from each rank, valid when the
+    packed rows are. The expert operators take these; the returned recv_count
+    is their sum over the ranks, which does not say where the rows lie."""
+
+    def __init__(self, topk_idx, num_tokens, plan_gen, recv_counts=None):
         self.topk_idx = topk_idx
         self.num_tokens = num_tokens
         self.plan_gen = plan_gen
+        self.recv_counts = recv_counts
 
 
 def _event():
@@ -121,10 +127,9 @@ class Buffer:
         nb.dispatch_send(x, topk_idx, reuse_plan=reuse)
         if not reuse:
             self._plan_gen += 1
-        handle = _Handle(topk_idx, x.shape[0], self._plan_gen)
-
         counts = torch.empty(nb.local_experts, nb.world, dtype=torch.int32,
                              device=x.device)
+        handle = _Handle(topk_idx, x.shape[0], self._plan_gen, counts)
         if use_fp8:
             packed = (nb.recv_x_view(), nb.recv_scale_view())
         else:

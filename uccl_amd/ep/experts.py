@@ -16,9 +16,10 @@ rows from row r * slots / sources on. Counts stay on the GPU; one below zero or
 above slots / sources counts as the nearest of the two. Rows behind the valid
 ones are neither read nor written: in a result that was passed as ``out`` they
 keep their values, in a fresh one they are undefined. ``counts=None``: all rows
-are valid; counts [experts] stands for one source (so the sums over ranks that
-``deep_ep_compat`` returns fit only where there is one rank). Two-dimensional
-operands are those of a single expert. At most 1024 experts and 2048 counts.
+are valid; counts [experts] stands for one source. ``deep_ep_compat`` returns
+sums over the ranks, which fit only where there is one rank: its handle's
+``recv_counts`` are the counts to pass. Two-dimensional operands are those of a
+single expert. At most 1024 experts and 2048 counts.
 A result shares no memory with an operand or the counts; it may lie between an
 operand's columns in a larger tensor.
 

@@ -12,6 +12,7 @@
 #include "../collective/communicator.h"
 #include "../core/log.h"
 #include "../ep/ep_buffer.h"
+#include "../ep/ep_proxy.h"
 #include "../p2p/endpoint.h"
 #include "../transport/reliable.h"
 #include "../p2p/compress.h"
@@ -329,6 +330,7 @@ PYBIND11_MODULE(_C, m) {
            py::call_guard<py::gil_scoped_release>());
 
   // --- EP (DeepEP-compatible expert parallel) -----------------------------
+  m.def("ep_proxy_lane_streams", &uccl::ep::EpProxy::lane_streams);
   py::class_<uccl::ep::EpBuffer>(m, "EpBuffer")
       .def(py::init([](int rank, int world, int device, int num_experts,
                        int topk, int hidden, int max_tokens, int elem_size,

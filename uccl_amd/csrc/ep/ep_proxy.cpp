@@ -96,27 +96,34 @@ struct TimedFlowLock {
   ~TimedFlowLock() { m.unlock(); }
 };
 
-// Lane copies must never queue behind the user's spin-wait kernels. HIP
-// gives a new stream a hardware queue of its own while it has one left
+// Lane copies must not queue behind the user's spin-wait kernels. HIP gives a
+// new stream a hardware queue of its own while it has one left
 // (GPU_MAX_HW_QUEUES, 4 by default) and lets further ones share, the null
-// stream's queue among them: with 5 lanes (world 4) and 4 queues a lane's
-// copy sat behind the dispatch wait that needed it, until that timed out.
-// So lanes take turns on at most queues - 1 streams, which live as long as
-// the process: a destroyed one would hand its queue to somebody else.
+// stream's queue among them: with 5 lanes (world 4) and 4 queues a lane's copy
+// sat behind the dispatch wait that needed it, until that timed out. So lanes
+// take turns on at most queues - 2 streams: the null stream and one stream
+// beside it keep queues of their own. A process that uses more streams needs
+// more queues; nothing here can see which queue a stream was given. The lanes'
+// streams live as long as the process: a destroyed one would hand its queue to
+// somebody else.
+int EpProxy::lane_streams() {
+  return static_cast<int>(
+      std::max<int64_t>(1, env_int("GPU_MAX_HW_QUEUES", 4) - 2));
+}
+
 static hipStream_t lane_stream(int device) {
   static std::mutex mu;
   static std::map<int, std::pair<std::vector<hipStream_t>, size_t>> pools;
   std::lock_guard<std::mutex> g(mu);
   auto& [streams, next] = pools[device];
-  size_t const most = static_cast<size_t>(
-      std::max<int64_t>(1, env_int("GPU_MAX_HW_QUEUES", 4) - 1));
+  size_t const most = static_cast<size_t>(EpProxy::lane_streams());
   if (streams.size() < most) {
     hipStream_t s = nullptr;
     UCCL_CHECK_HIP(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
     streams.push_back(s);
     return s;
   }
-  return streams[next++ % most];
+  return streams[next++ % streams.size()];
 }
 
 EpProxy::Lane::Lane(int device, size_t bytes) {

@@ -48,6 +48,9 @@ class EpProxy {
 
   void start();
 
+  // Streams that the lanes of all proxies of a device share.
+  static int lane_streams();
+
  private:
   struct WireHdr {
     uint32_t kind;   // 1=dispatch, 2=combine, 3=combine-done,

@@ -60,15 +60,14 @@ int EpProxy::flow_peer(uint64_t flow) const {
   return 0;
 }
 
-// A flow mutex held for seconds means another lane is wedged mid-ship;
-// log instead of blocking invisibly (a silent block here produced
-// "last expert never shipped" stalls that were unattributable).
-// hipStreamSynchronize that logs instead of blocking invisibly: a lane
+// Waits for this lane's own copies: lanes share streams, and other lanes' later
+// copies are none of its business. Logs instead of blocking invisibly: a lane
 // sync stuck for seconds means the copy engine / device is wedged.
-static void lane_sync(hipStream_t stream, char const* who) {
+void EpProxy::lane_sync(Lane& lane, char const* who) {
+  UCCL_CHECK_HIP(hipEventRecord(lane.done, lane.stream));
   auto const t0 = std::chrono::steady_clock::now();
   for (;;) {
-    hipError_t const e = hipStreamQuery(stream);
+    hipError_t const e = hipEventQuery(lane.done);
     if (e == hipSuccess) return;
     if (e != hipErrorNotReady) {
       UCCL_CHECK_HIP(e);
@@ -80,13 +79,22 @@ static void lane_sync(hipStream_t stream, char const* who) {
     if (el > 5.0) {
       UCCL_LOG_WARN << "ep proxy lane sync stalled " << el << "s (" << who
                     << ")";
-      (void)hipStreamSynchronize(stream);
+      (void)hipEventSynchronize(lane.done);
       return;
     }
     usleep(50);
   }
 }
 
+// The same without the pause between looks.
+void EpProxy::lane_wait(Lane& lane) {
+  UCCL_CHECK_HIP(hipEventRecord(lane.done, lane.stream));
+  UCCL_CHECK_HIP(hipEventSynchronize(lane.done));
+}
+
+// A flow mutex held for seconds means another lane is wedged mid-ship;
+// log instead of blocking invisibly (a silent block here produced
+// "last expert never shipped" stalls that were unattributable).
 struct TimedFlowLock {
   std::timed_mutex& m;
   TimedFlowLock(std::timed_mutex& mu, char const* who) : m(mu) {
@@ -129,6 +137,7 @@ static hipStream_t lane_stream(int device) {
 EpProxy::Lane::Lane(int device, size_t bytes) {
   UCCL_CHECK_HIP(hipSetDevice(device));
   stream = lane_stream(device);
+  UCCL_CHECK_HIP(hipEventCreateWithFlags(&done, hipEventDisableTiming));
   UCCL_CHECK_HIP(hipHostMalloc(&buf, bytes));
   UCCL_CHECK_HIP(hipHostMalloc(&buf2, bytes));
 }
@@ -136,6 +145,7 @@ EpProxy::Lane::Lane(int device, size_t bytes) {
 EpProxy::Lane::~Lane() {
   if (buf) (void)hipHostFree(buf);
   if (buf2) (void)hipHostFree(buf2);
+  if (done) (void)hipEventDestroy(done);
 }
 
 EpProxy::EpProxy(const EpView& view, void* heap, D2HRing* ring_host,
@@ -239,7 +249,7 @@ void EpProxy::ship_rows(Lane& lane, uint64_t flow, WireHdr const& h,
     size_t const n0 = std::min(stage_bytes_, total);
     UCCL_CHECK_HIP(hipMemcpyAsync(bufs[cur], dev_rows, n0,
                                   hipMemcpyDeviceToHost, lane.stream));
-    lane_sync(lane.stream, "ship first d2h");
+    lane_sync(lane, "ship first d2h");
   }
   while (off < total) {
     size_t const n = std::min(stage_bytes_, total - off);
@@ -251,7 +261,7 @@ void EpProxy::ship_rows(Lane& lane, uint64_t flow, WireHdr const& h,
           hipMemcpyDeviceToHost, lane.stream));
     }
     tp_->send_msg(flow, bufs[cur], n);
-    if (next_off < total) lane_sync(lane.stream, "ship next d2h");
+    if (next_off < total) lane_sync(lane, "ship next d2h");
     off = next_off;
     cur ^= 1;
   }
@@ -264,7 +274,7 @@ void EpProxy::ship_rows(Lane& lane, uint64_t flow, WireHdr const& h,
       UCCL_CHECK_HIP(hipMemcpyAsync(
           lane.buf, static_cast<char const*>(dev_scales) + soff, n,
           hipMemcpyDeviceToHost, lane.stream));
-      lane_sync(lane.stream, "ship scales d2h");
+      lane_sync(lane, "ship scales d2h");
       tp_->send_msg(flow, lane.buf, n);
       soff += n;
     }
@@ -277,7 +287,7 @@ void EpProxy::ship_rows(Lane& lane, uint64_t flow, WireHdr const& h,
     UCCL_CHECK_HIP(hipMemcpyAsync(metas.data(), dev_metas_or_null,
                                   h.count * sizeof(uint32_t),
                                   hipMemcpyDeviceToHost, lane.stream));
-    lane_sync(lane.stream, "ship metas d2h");
+    lane_sync(lane, "ship metas d2h");
   }
   if (h.count)
     tp_->send_msg_async(flow, metas.data(), h.count * sizeof(uint32_t));
@@ -318,7 +328,7 @@ void EpProxy::ship_batch(Lane& lane, uint64_t flow, uint32_t seq,
     size_t const n0 = std::min(stage_bytes_, total);
     UCCL_CHECK_HIP(hipMemcpyAsync(bufs[cur], dev_rows, n0,
                                   hipMemcpyDeviceToHost, lane.stream));
-    lane_sync(lane.stream, "batch first d2h");
+    lane_sync(lane, "batch first d2h");
   }
   while (off < total) {
     size_t const n = std::min(stage_bytes_, total - off);
@@ -329,7 +339,7 @@ void EpProxy::ship_batch(Lane& lane, uint64_t flow, uint32_t seq,
                                     hipMemcpyDeviceToHost, lane.stream));
     }
     tp_->send_msg(flow, bufs[cur], n);
-    if (next_off < total) lane_sync(lane.stream, "batch next d2h");
+    if (next_off < total) lane_sync(lane, "batch next d2h");
     off = next_off;
     cur ^= 1;
   }
@@ -343,7 +353,7 @@ void EpProxy::ship_batch(Lane& lane, uint64_t flow, uint32_t seq,
       size_t const n = std::min(stage_bytes_, stotal - soff);
       UCCL_CHECK_HIP(hipMemcpyAsync(lane.buf, dev_scales + soff, n,
                                     hipMemcpyDeviceToHost, lane.stream));
-      lane_sync(lane.stream, "batch scales d2h");
+      lane_sync(lane, "batch scales d2h");
       tp_->send_msg(flow, lane.buf, n);
       soff += n;
     }
@@ -354,7 +364,7 @@ void EpProxy::ship_batch(Lane& lane, uint64_t flow, uint32_t seq,
                                   egress_meta(heap_, v_, row0),
                                   total_rows * sizeof(uint32_t),
                                   hipMemcpyDeviceToHost, lane.stream));
-    lane_sync(lane.stream, "batch metas d2h");
+    lane_sync(lane, "batch metas d2h");
     tp_->send_msg_async(flow, metas.data(), total_rows * sizeof(uint32_t));
   }
   tp_->flush_sends(flow);
@@ -370,7 +380,7 @@ int EpProxy::num_proxy_peers() const {
 void EpProxy::write_sync_flag(Lane& lane, int idx, uint64_t seq) {
   UCCL_CHECK_HIP(hipMemcpyAsync(sync_ptr(heap_, v_, idx), &seq, sizeof(seq),
                                 hipMemcpyHostToDevice, lane.stream));
-  UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+  lane_wait(lane);
 }
 
 // one arrival (self or a peer's kBar message) for barrier `seq`; when
@@ -631,7 +641,7 @@ void EpProxy::comb_tx_loop() {
             ++le;
           }
           if (!rows) continue;  // all-empty group: nothing to carry
-          lane_sync(lane.stream, "comb gather d2h");
+          lane_sync(lane, "comb gather d2h");
           WireHdr h{kComb, static_cast<uint32_t>(task.seq),
                     static_cast<uint32_t>(le0),
                     static_cast<uint32_t>(v_.rank), rows};
@@ -709,7 +719,7 @@ void EpProxy::rx_loop(int peer) {
         UCCL_CHECK_HIP(hipMemcpyAsync(consumed_ptr(heap_, v_, peer), &seq,
                                       sizeof(seq), hipMemcpyHostToDevice,
                                       lane.stream));
-        lane_sync(lane.stream, "consume h2d");
+        lane_sync(lane, "consume h2d");
         continue;
       }
       if (h.kind == kAtom) {
@@ -720,17 +730,17 @@ void EpProxy::rx_loop(int peer) {
         char* addr = static_cast<char*>(heap_) + h.aux;
         UCCL_CHECK_HIP(hipMemcpyAsync(&cur, addr, sizeof(cur),
                                       hipMemcpyDeviceToHost, lane.stream));
-        UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+        lane_wait(lane);
         cur += h.count;
         UCCL_CHECK_HIP(hipMemcpyAsync(addr, &cur, sizeof(cur),
                                       hipMemcpyHostToDevice, lane.stream));
-        UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+        lane_wait(lane);
         continue;
       }
       if (h.kind == kCombDone) {
         // all combine payloads from `peer` for this seq have been
         // scattered (lane.stream is in-order); publish the flag
-        UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+        lane_wait(lane);
         // NB: must NOT use the legacy default stream here — it would wait
         // for the peer's spinning wait-kernel (deadlock). lane.stream is
         // non-blocking.
@@ -738,7 +748,7 @@ void EpProxy::rx_loop(int peer) {
         UCCL_CHECK_HIP(hipMemcpyAsync(comb_flag_ptr(heap_, v_, peer), &seq,
                                       sizeof(seq), hipMemcpyHostToDevice,
                                       lane.stream));
-        UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+        lane_wait(lane);
         continue;
       }
       if (h.kind == kDispB) {
@@ -787,7 +797,7 @@ void EpProxy::rx_loop(int peer) {
                   hipMemcpyHostToDevice, lane.stream));
               done += span;
             }
-            lane_sync(lane.stream, "batch rows h2d");
+            lane_sync(lane, "batch rows h2d");
             off += n;
           }
         };
@@ -821,7 +831,7 @@ void EpProxy::rx_loop(int peer) {
           UCCL_CHECK_HIP(hipMemcpyAsync(
               disp_count_ptr(heap_, v_, le, h.src), &tagged,
               sizeof(tagged), hipMemcpyHostToDevice, lane.stream));
-          lane_sync(lane.stream, "batch tag h2d");
+          lane_sync(lane, "batch tag h2d");
         }
         continue;
       }
@@ -841,7 +851,7 @@ void EpProxy::rx_loop(int peer) {
         tp_->recv_msg(flow, lane.buf, n);
         UCCL_CHECK_HIP(hipMemcpyAsync(dev_dst + off, lane.buf, n,
                                       hipMemcpyHostToDevice, lane.stream));
-        UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+        lane_wait(lane);
       }
       if (fp8_disp && h.count) {
         // second stream: per-row scales into the contiguous scale span
@@ -855,7 +865,7 @@ void EpProxy::rx_loop(int peer) {
           UCCL_CHECK_HIP(hipMemcpyAsync(sdst + off, lane.buf, n,
                                         hipMemcpyHostToDevice,
                                         lane.stream));
-          lane_sync(lane.stream, "disp scales h2d");
+          lane_sync(lane, "disp scales h2d");
         }
       }
       metas.resize(h.count);
@@ -867,13 +877,13 @@ void EpProxy::rx_loop(int peer) {
                           static_cast<size_t>(h.src) * v_.max_tokens),
             metas.data(), h.count * sizeof(uint32_t),
             hipMemcpyHostToDevice, lane.stream));
-        UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+        lane_wait(lane);
         uint64_t const tagged =
             (static_cast<uint64_t>(h.seq32) << 32) | h.count;
         UCCL_CHECK_HIP(hipMemcpyAsync(disp_count_ptr(heap_, v_, h.le, h.src),
                                       &tagged, sizeof(tagged),
                                       hipMemcpyHostToDevice, lane.stream));
-        UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+        lane_wait(lane);
       } else {  // kComb: scatter ingress rows into comb_x cells by meta
         if (h.count) {
           UCCL_CHECK_HIP(hipMemcpyAsync(ingress_meta(heap_, v_, ing0),
@@ -881,7 +891,7 @@ void EpProxy::rx_loop(int peer) {
                                         h.count * sizeof(uint32_t),
                                         hipMemcpyHostToDevice, lane.stream));
           launch_ep_comb_scatter(v_, ing0, h.count, lane.stream);
-          UCCL_CHECK_HIP(hipStreamSynchronize(lane.stream));
+          lane_wait(lane);
         }
       }
     }

@@ -71,10 +71,13 @@ class EpProxy {
     void* buf2 = nullptr;  // double buffer: D2H of chunk i+1 overlaps the
                            // transport send of chunk i (batched posting)
     hipStream_t stream = nullptr;
+    hipEvent_t done = nullptr;
     Lane(int device, size_t bytes);
     ~Lane();
   };
 
+  static void lane_sync(Lane& lane, char const* who);
+  static void lane_wait(Lane& lane);
   void ring_loop();
   void rx_loop(int peer);
   void comb_tx_loop();

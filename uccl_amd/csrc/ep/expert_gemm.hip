@@ -1351,41 +1351,80 @@ void launch_long(GemmArgs const& a, int expected_rows, hipStream_t s) {
 }
 
 // Which kernel, by the rows that an expert is expected to have and the tiles
-// that this makes. Measured in us:
-//   32 experts, 4096 x 7168, 8 bits      rows:   8    16    32    64   128
-//     k_expert_rows                            171   212   284
-//     tiles of 256 x 64                                    172   215   309
-//     tiles of 256 x 128                                   190   197   256
-//     tiles of 256 x 256                       252   255   253   266   271
-//   the same, rows on average, experts     10    24    32    48    94   128
-//   of unlike popularity
-//     tiles of 256 x 64                     159   169   209   201   251   303
-//     tiles of 256 x 128                    180   170   172   177   238   247
-//     tiles of 256 x 256                    265   253   260   250   265   258
+// that this makes. Measured in us, as calls in a stream, experts of unlike
+// popularity, rows of an expert on average:
+//                      rows   1   2   4   8  16  24  32  48  64  96 128 192 256
+//   8 bits, 32 experts, 4096 x 7168
+//     k_expert_rows         106 134 165 171 213 252 290
+//     tiles of 256 x 64     134 141 161 153 165 168 208 202 206 253 302 403
+//     tiles of 256 x 128    140 150 165 159 167 170 173 178 223 233 238 300 405
+//     tiles of 256 x 256    193 206 233 226 237 241 241 240 244 251 253 326 361
+//   8 bits, 16 experts, 7168 x 2048
+//     k_expert_rows          36  39  48  60  70  77  90
+//     tiles of 256 x 64      39  39  40  41  42  42  43  61  62  76  94 128
+//     tiles of 256 x 128     40  40  40  42  43  43  46  46  48  64  67  88 111
+//     tiles of 256 x 256     56  57  57  60  63  63  63  65  63  67  68  98 106
+//   8 bits, 8 experts, 4096 x 4096: 128 tiles of 256 x 64, half of the card
+//     k_expert_rows          24  26  27  31  36  42  57
+//     tiles of 256 x 64      34  35  35  35  35  36  36  37  37  38  68  69
+//     tiles of 256 x 128     34  36  36  36  36  36  37  37  37  38  40  43  70
+//     tiles of 256 x 256                                         52  53  56  58
+//   16 bits, 32 experts, 4096 x 7168
+//     k_expert_rows         192 251 313 309 375 441 513
+//     tiles of 256 x 64     238 257 308 291 313 316 376 356 360 418 485 633
+//     tiles of 256 x 128    250 270 309 294 313 316 319 325 401 398 404 512 682
+//     tiles of 256 x 256    324 366 419 403 419 422 422 424 428 432 435 560 608
+//   16 bits, 16 experts, 7168 x 2048
+//     k_expert_rows          55  66  79 100 116 127 144
+//     tiles of 256 x 64      65  80  96 111 111 112 111 124 123 132 158 197
+//     tiles of 256 x 128     70  86  99 114 116 115 116 118 117 134 135 156 188
+//     tiles of 256 x 256     95 103 116 126 127 128 128 130 132 135 137 171 182
+//   16 bits, 8 experts, 4096 x 4096
+//     k_expert_rows          35  46  47  47  55  62  84
+//     tiles of 256 x 64      46  48  48  47  49  50  50  52  54  59  98 105
+//     tiles of 256 x 128     55  56  58  57  58  58  59  59  60  65  68  75 124
+//     tiles of 256 x 256                                         91  92 102 102
+//   the same turned (row gradients), 16 experts, 7168 x 2048
+//     tiles of 256 x 64      65  70  78  85  87  89  89 108 109 124 150 191
+//     tiles of 256 x 128     72  77  84  91  92  93  93  96  95 123 125 152 186
+//     tiles of 256 x 256     98 101 106 118 119 121 121 120 125 126 127 169 172
 //   1 expert, 7168 x 2048, 8 bits        rows:   1    16    64
 //     k_expert_rows                            5.5   7.6  16.4
 //     tiles of 128 x 128                      20.0  20.1  20.4
+// Few tiles, experts of like popularity, one round of 128 x 128 or less:
 //   128 rows of 4 / 8 experts   512 x 1024, 16 bits   1024 x 1024, 8 bits
 //     k_expert_rows                    8.4 / 13.0           10.3 / 18.5
 //     tiles of 128 x 128              14.3 / 14.5           12.5 / 12.9
-//   8 experts, 256 rows    1024 x 1024, 16 bits   2048 x 1024, 8 bits
-//     tiles of 128 x 128                  15.2                   26.4
-//     tiles of 256 x 128                  19.9                   16.4
-//   weight gradient, 8 experts, 139 rows  1000 x 1024, 16 bits
-//     tiles of 128 x 128                  17.2
-//     tiles of 256 x 128                  12.5
-//     tiles of 256 x 256                  15.8
-//     k_expert_long                       46.5
-//   the same, n x k (experts, rows)  56 x 72   512 x 512   512 x 512  88 x 3544
-//                                   (2, 1623)   (8, 139)   (8, 2500) (3, 3345)
-//     tiles of 256 x 128               32.6       10.3        51.7       66.4
-//     k_expert_long                    11.9       12.5        43.3       44.1
-//   row gradient, 128 rows           512 x 1024 of 4 / 8 experts
-//     tiles of 128 x 128               14.8 / 15.0
-//     k_expert_long                    10.3 / 10.5
-//   row gradient, 6 rows of 32 experts, 1024 x 512
-//     tiles of 256 x 64                10.5
-//     k_expert_long                    14.2
+//   tiles of 128 x 128:            128, 8 bits  128, 16 bits  256 to 280, 8 bits
+//     8 experts x 200, 1024 x 1024  13.2 / 14.0  14.9 / 19.0
+//     4 experts x 200, 2048 x 2048  20.4 / 21.2  23.9 / 31.4
+//     16 experts x 200, 512 x 1024  13.1 / 14.1  15.1 / 19.0
+//     2 experts x 200, 4096 x 1024  13.0 / 14.2  14.7 / 18.9
+//     8 experts x 200, 2048 x 1024                            24.4 / 15.1
+//   with 128 x 128 / 256 x 128; 8 bits fit once on a compute unit, so that the
+//   odd tile more than there are units costs a round. (16 bits, 8 x 200 and
+//   8 x 512 rows, 2048 x 1024: 19.9 / 20.2 and 29.6 / 35.9.)
+//   row gradients, k_expert_long / tiles of 128 x 128, by tiles of 64 x 64
+//                       tiles  64 or less     128            192         256
+//     8 experts, 512 x 1024    7.6 / 14.2   9.5 / 14.5   9.7 / 14.9
+//     8 experts, 1024 x 1024                7.9 / 14.4               9.8 / 14.7
+//     4 experts, 1024 x 2048  10.7 / 23.6  13.9 / 23.9  15.1 / 24.4
+//     3 experts, 1000 x 4096  20.2 / 42.2
+//     16 experts, 512 x 512                 6.4 /  9.5               7.5 /  9.8
+//     8 experts, 1024 x 256                 6.2 /  7.0               6.5 /  7.4
+//   (up to 9.7 / 7.4 where an expert has more rows than expected), 384: 16.7 /
+//   15.3, 12.8 / 10.3
+//   weight gradients, k_expert_long / tiles of 256 x 128
+//                         rows      139         512        2048        4096
+//     256 tiles of 64 x 64
+//       4 experts, 512 x 512     6.0 /  9.8  8.2 / 16.3 18.7 / 42.5 30.9 / 77.4
+//       1 expert, 1024 x 1024    6.0 /  9.8  7.1 / 14.1 14.6 / 36.7 23.8 / 67.1
+//       64 experts, 128 x 128    6.1 /  9.6  8.4 / 17.0 21.3 / 45.1 37.4 / 82.4
+//     512 tiles
+//       8 experts, 512 x 512    10.7 / 10.1 16.5 / 16.6 37.0 / 44.2 65.0 / 79.6
+//       2 experts, 1024 x 1024  10.5 / 10.2 14.4 / 15.9 29.8 / 40.8 47.9 / 72.8
+//     8 experts, 1000 x 1024    46.5 / 12.5 (256 x 256 15.8)
+//     3 experts x 3345 rows, 88 x 3544 (336 tiles): 44.1 / 66.4
 template <Mode kMode, Elem kElem, Elem kOut>
 void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
   auto tiles = [&](int p, int q) {
@@ -1394,7 +1433,9 @@ void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
   };
   int const cus = compute_units();
   if constexpr (kMode == Mode::kProduct) {
-    if (expected_rows <= 16 || tiles(16, 64) <= 2 * cus) {
+    int const few =
+        kElem != Elem::kF8 ? 8 : tiles(256, 64) >= cus ? 2 : 16;
+    if (expected_rows <= few || tiles(16, 64) <= 2 * cus) {
       if (tiles(32, 64) >= 4 * cus)
         launch_rows<kElem, kOut, 2>(a, expected_rows, s);
       else
@@ -1417,7 +1458,7 @@ void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
       return launch_tiles<kMode, kElem, kOut, 128, 128, 2, 2>(a, 2, s);
     if (expected_rows <= 24)
       return launch_tiles<kMode, kElem, kOut, 256, 64, 4, 1>(a, 1, s);
-    if (expected_rows <= 96)
+    if (expected_rows <= 192)
       return launch_tiles<kMode, kElem, kOut, 256, 128, 4, 2>(a, 1, s);
   }
   if (tiles(256, 256) >= cus)

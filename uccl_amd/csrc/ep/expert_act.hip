@@ -19,7 +19,8 @@
 // 8 bits: scales and values are those of exact arithmetic, whatever the last
 // bits of a float exponential are. Only the largest |v| of a group is worked
 // out in 64 bits, and values that lie so close to the middle between two 8-bit
-// values that 32 bits do not decide; groups outside 1e-30 .. 1e30 entirely.
+// values that 32 bits do not decide; groups whose largest |v| is outside
+// 1e-20 .. 1e30, or that have a below -85, entirely.
 
 #include <hip/hip_runtime.h>
 
@@ -299,8 +300,9 @@ __global__ __launch_bounds__(256) void k_swiglu_quant(SwigluArgs a) {
                               [&](Share const (&s)[kShares], Data const& raw) {
     // a group's 128 columns are 16 neighbouring lanes, all of them on or off
     f32x8 v[kShares];
-    // v in 32 bits, good to (|a| + 6) 2^-24 of its size: an exponential of a
-    // rounded product and five operations more. Groups with a below -85,
+    // v in 32 bits, good to 70 parts in 2^24 for a down to -85: 64 of the
+    // exponential (its argument is rounded, up to 45, and so is log2(e) in
+    // it, 0.22 |a|) and one of each operation more. Groups with a below -85,
     // where the exponential ends, or whose largest |v| is far from 1 are
     // `wild`: nothing of them is decided in 32 bits.
     bool wild[kShares];

@@ -38,7 +38,6 @@
 #include <type_traits>
 
 #include "../core/log.h"
-#include "../device/primitives.h"
 #include "expert_ops.h"
 
 // The loads below list m0 as clobbered, which is what tells the compiler that
@@ -54,7 +53,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -352,8 +350,6 @@ __device__ __forceinline__ Tile find_tile(GemmArgs const& a,
   return r;
 }
 
-constexpr int less(int a, int b) { return a < b ? a : b; }
-
 template <int kH>
 __device__ __forceinline__ i32x4 half(i32x8 v) {
   return __builtin_shufflevector(v, v, kH * 4, kH * 4 + 1, kH * 4 + 2,
@@ -405,7 +401,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void k_expert_gemm(GemmArgs a) {
   __shared__ float p_scale[k8 ? 4 : 1][k8 ? 64 : 1];
   __shared__ RowTable table;
   // rows of a tile: of the last, whose results are stored, of this one and of
-  // the next; weight gradient: rows of a stage, 4 stages in a ring
+  // the next; weight gradient: rows of a stage, kNoted stages in a ring
   constexpr int kNoted = 8;
   __shared__ int slots[kWGrad ? kNoted : 3][kWGrad ? kDepth : BQ];
   __shared__ uint32_t p_rows[kWGrad ? kNoted : 1][kWGrad ? kDepth : 1];

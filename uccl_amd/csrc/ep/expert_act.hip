@@ -7,14 +7,15 @@
 //
 // Every value is read and written once, 16 bytes a lane and load; a wave takes
 // 512 columns of a row, or several rows of fewer columns. 16 bits are bound by
-// memory: 16384 rows of 2048 columns, 47 us, 4.3 TB/s, and 74 us, 4.5 TB/s, for
+// memory: 16384 rows of 2048 columns, 48 us, 4.2 TB/s, and 74 us, 4.5 TB/s, for
 // the gradient. 8 bits are bound by the vector units, about 39 instructions a
-// value: 32768 rows of 2048 columns, 109 us, 3.1 TB/s.
+// value: 32768 rows of 2048 columns, 111 us, 3.0 TB/s.
 //
 // The exponential is taken of -|a| / 2 and used twice, w = exp(-|a| / 2): for
 // a < 0 sig(a) = w w / (1 + w w), and the factors of a product take one w
-// each, so nothing overflows and no product of normal size is lost to an
-// underflow on the way.
+// each, so nothing overflows, and no product above 6e-36 is lost to an
+// underflow on the way (w ends at a = -174.6, where a |b| of 1e36 and more
+// would still give a normal one).
 //
 // 8 bits: scales and values are those of exact arithmetic, whatever the last
 // bits of a float exponential are. Only the largest |v| of a group is worked

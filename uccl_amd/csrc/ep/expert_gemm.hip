@@ -25,12 +25,14 @@
 // What bounds a large product is LDS: a step of a 256 x 256 tile brings 64 KB
 // in and gives 192 KB to the waves, 2048 clocks of the 128 bytes it moves in
 // each, and the same 2048 clocks the matrix units are busy. 16384 rows of 8
-// experts, bf16: product 7168 x 4096 806 us, 1.19 PFLOP/s, its row gradient
-// 830 us, weight gradient 4096 x 7168 848 us, 1.13 PFLOP/s; 32768 rows, 4096 x
-// 7168, 8 bits: 917 us, 2.10 PFLOP/s. (The card's library reaches 1.40 and
-// 2.73 on dense products of 8192 cubed.) Products of few rows are bound by the
-// weights' bytes: 1024 rows of 32 experts, 4096 x 7168, 8 bits: 171 us, 5.5
-// TB/s.
+// experts, bf16, calls in a stream on several cards, the slowest of which is 7%
+// behind the fastest: product 7168 x 4096 805 us, 1.20 PFLOP/s, its row
+// gradient 815 to 885 us, weight gradient 4096 x 7168 865 to 924 us, 1.04 to
+// 1.11 PFLOP/s; 32768 rows, 4096 x 7168, 8 bits: 906 to 969 us, 1.99 to 2.12
+// PFLOP/s. (The library reaches 1.40 and 2.73 on dense products of 8192 cubed,
+// on the fastest 1.55 and 3.10.) Products of few rows are bound by the
+// weights' bytes: 1024 rows of 32 experts, 4096 x 7168, 8 bits: 175 to 179 us,
+// 5.4 TB/s, bf16: 322 us, 5.9 TB/s.
 
 #include <hip/hip_runtime.h>
 

@@ -4,10 +4,12 @@ Between the router's logits and ``combine``, on one rank:
 
     idx, weights = ep.route(logits, topk)
     recv_x, counts, recv_scales = buf.dispatch(x, idx)          # use_fp8=True
-    h = ep.expert_matmul(recv_x, w13, counts,
-                         x_scales=recv_scales, w_scales=w13_scales)
+    rows = -(-len(x) * buf.world * topk // buf.num_experts)     # on average
+    h = ep.expert_matmul(recv_x, w13, counts, x_scales=recv_scales,
+                         w_scales=w13_scales, expected_rows=rows)
     a, a_scales = ep.expert_swiglu(h, counts, quantize=True)
-    y = ep.expert_matmul(a, w2, counts, x_scales=a_scales, w_scales=w2_scales)
+    y = ep.expert_matmul(a, w2, counts, x_scales=a_scales,
+                         w_scales=w2_scales, expected_rows=rows)
     out = buf.combine(y, idx, weights)
 
 A slot array is [experts, slots, columns]; with counts [experts, sources]
@@ -19,9 +21,9 @@ keep their values, in a fresh one they are undefined. ``counts=None``: all rows
 are valid; counts [experts] stands for one source. ``deep_ep_compat`` returns
 sums over the ranks, which fit only where there is one rank: its handle's
 ``recv_counts`` are the counts to pass. Two-dimensional operands are those of a
-single expert. At most 1024 experts and 2048 counts.
-A result shares no memory with an operand or the counts; it may lie between an
-operand's columns in a larger tensor.
+single expert. At most 1024 experts and 2048 counts. A result shares no memory
+with an operand or the counts; it may lie between an operand's columns in a
+larger tensor.
 
 Every call is enqueued on the current stream of its operands' device and may be
 captured into a graph. Operands lie on one device; rows start at 16-byte
@@ -154,8 +156,10 @@ def expert_matmul(x: torch.Tensor, w: torch.Tensor,
     as it lies (its N, the weights' K, a multiple of 8).
 
     ``expected_rows``: how many rows an expert is expected to have, by which
-    the kernel is chosen (default: all its slots). It changes the speed and
-    the order of the sums, never which rows are computed.
+    the kernel is chosen. It changes the speed and the order of the sums, never
+    which rows are computed. Without it all slots are expected, which suits
+    full ones: 32 rows of 32 experts each, 4096 x 7168, take 238 us instead of
+    175 in 8 bits, 420 instead of 322 in 16.
     """
     C = _native(x=x, w=w, x_scales=x_scales, w_scales=w_scales, out=out)
     if out is None:

@@ -51,3 +51,31 @@ def test_limits_of_expected_rows(e, n, kind, expected):
     bad = (y.double() - want).abs() > want.abs() * 2.0 ** -8 + size * off
     assert not bad[mask].any()
     assert (y[~mask] == 7).all()
+
+
+@pytest.mark.parametrize("expected", [2, 3, 16, 17, 32, 33])
+@pytest.mark.parametrize("precise", [False, True])
+def test_limits_where_8_bit_rows_lie_far_apart(precise, expected):
+    """Rows that a tile's 32-bit offsets do not reach, shared by all experts."""
+    g = torch.Generator(device="cuda").manual_seed(expected)
+    e, slots, n, k = 40, 300, 1032, 256
+    room = torch.empty(slots << 24, dtype=torch.uint8, device="cuda").view(F8)
+    x = room.view(1, slots, 1 << 24)[..., :k]
+    x.copy_((torch.randn(1, slots, k, device="cuda", generator=g) * 50).to(F8))
+    x = x.expand(e, slots, k)
+    w = (torch.randn(e, n, k, device="cuda", generator=g) * 50).to(F8)
+    xs = torch.full((e, slots, 2), 0.0625, device="cuda")
+    ws = torch.full((e, 9, 2), 0.125, device="cuda")
+    counts = torch.randint(0, 2 * expected + 1, (e, 1), device="cuda",
+                           generator=g, dtype=torch.int32)
+    mask = torch.arange(slots, device="cuda") < counts
+    y = torch.full((e, slots, n), 7.0, dtype=BF, device="cuda")
+    ep.expert_matmul(x, w, counts, x_scales=xs, w_scales=ws, out=y,
+                     expected_rows=expected, precise=precise)
+    x, wt = x.double(), w.double().transpose(1, 2).contiguous()
+    want = torch.matmul(x.contiguous(), wt) * 2.0 ** -7
+    size = torch.matmul(x.abs().contiguous(), wt.abs()) * 2.0 ** -7
+    off = (k + 3) * 2.0 ** -23 + (0.0 if precise else 2.0 ** -13)
+    bad = (y.double() - want).abs() > want.abs() * 2.0 ** -8 + size * off
+    assert not bad[mask].any()
+    assert (y[~mask] == 7).all()

@@ -1389,6 +1389,10 @@ void launch_long(GemmArgs const& a, int expected_rows, hipStream_t s) {
 //   1 expert, 7168 x 2048, 8 bits        rows:   1    16    64
 //     k_expert_rows                            5.5   7.6  16.4
 //     tiles of 128 x 128                      20.0  20.1  20.4
+//   32 experts, 4096 x 7168, 8 bits, rows too far apart for 32-bit offsets
+//     k_expert_rows                    rows:   1   4   8  16  32
+//                                            154 159 178 238 332
+//     tiles of 128 x 128                     409 410 409 409 410
 // Few tiles, experts of like popularity, one round of 128 x 128 or less:
 //   128 rows of 4 / 8 experts   512 x 1024, 16 bits   1024 x 1024, 8 bits
 //     k_expert_rows                    8.4 / 13.0           10.3 / 18.5
@@ -1431,8 +1435,10 @@ void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
   };
   int const cus = compute_units();
   if constexpr (kMode == Mode::kProduct) {
-    int const few =
-        kElem != Elem::kF8 ? 8 : tiles(256, 64) >= cus ? 2 : 16;
+    int const few = kElem != Elem::kF8        ? 8
+                    : !a.near                 ? 32
+                    : tiles(256, 64) >= cus   ? 2
+                                              : 16;
     if (expected_rows <= few || tiles(16, 64) <= 2 * cus) {
       if (tiles(32, 64) >= 4 * cus)
         launch_rows<kElem, kOut, 2>(a, expected_rows, s);
@@ -1481,6 +1487,9 @@ void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
 //     k_expert_rows                          25   32   36   43   79
 //     tiles of 256 x 64                      49   49   49   49   50   50   53   97
 //     tiles of 256 x 128                     60   61   60   61   61   62   61   63
+//   32 experts, 4096 x 7168, rows too far apart for 32-bit offsets
+//     k_expert_rows                         192       211  238  516
+//     tiles of 128 x 128                    512       512  513  513
 template <Elem kOut>
 void launch_wide(GemmArgs const& a, int expected_rows, hipStream_t s) {
   constexpr Mode kMode = Mode::kProduct;
@@ -1490,8 +1499,8 @@ void launch_wide(GemmArgs const& a, int expected_rows, hipStream_t s) {
            ((expected_rows + q - 1) / q);
   };
   int const cus = compute_units();
-  if (expected_rows <= (tiles(256, 64) < cus ? 8 : 2) ||
-      tiles(16, 64) <= 2 * cus)
+  int const few = !a.near ? 32 : tiles(256, 64) < cus ? 8 : 2;
+  if (expected_rows <= few || tiles(16, 64) <= 2 * cus)
     launch_rows<kElem, kOut, 1, Sums::k32>(a, expected_rows, s);
   else if (!a.near)
     launch_tiles<kMode, kElem, kOut, 128, 128, 2, 2, true, Sums::k32>(a, 2, s);

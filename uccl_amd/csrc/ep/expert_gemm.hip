@@ -1435,10 +1435,10 @@ void launch_sized(GemmArgs const& a, int expected_rows, hipStream_t s) {
   };
   int const cus = compute_units();
   if constexpr (kMode == Mode::kProduct) {
-    int const few = kElem != Elem::kF8        ? 8
-                    : !a.near                 ? 32
-                    : tiles(256, 64) >= cus   ? 2
-                                              : 16;
+    int const few = kElem != Elem::kF8      ? 8
+                    : !a.near               ? 32
+                    : tiles(256, 64) >= cus ? 2
+                                            : 16;
     if (expected_rows <= few || tiles(16, 64) <= 2 * cus) {
       if (tiles(32, 64) >= 4 * cus)
         launch_rows<kElem, kOut, 2>(a, expected_rows, s);
